@@ -1,0 +1,83 @@
+// Shared by the drafted-token operators (head_rows.hip, tree_attn.hip, sample_rows.hip): element types of device tensors,
+// 8-element loads and stores, division by a run-time constant, and the launch that reports its own error.
+#pragma once
+#include "common.h"
+#include "funasr_hip.h"
+
+namespace fa {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+template <typename T> struct Vec8;
+template <> struct Vec8<_Float16> { typedef f16x8_t type; };
+template <> struct Vec8<__bf16> { typedef bf16x8_t type; };
+
+// eight consecutive elements as floats; VEC: the address is 16-byte aligned
+template <bool VEC, typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+    const auto v = *reinterpret_cast<const typename Vec8<T>::type*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+  }
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = (T)x[i];
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (T)x[i];
+    *reinterpret_cast<typename Vec8<T>::type*>(p) = v;
+  }
+}
+
+// x / d for 0 <= x < 2^31 and a divisor 1 <= d < 2^31 that only the host knows beforehand: with s = ceil(log2 d) and
+// m = floor(2^(31 + s) / d) + 1 <= 2^32, x m / 2^(31 + s) exceeds x / d by at most x / 2^(31 + s) < 1 / d, so the floors agree.
+struct FastDiv {
+  uint64_t mul = 0;
+  uint32_t shift = 0, d = 1;
+  static FastDiv of(uint32_t d) {
+    FastDiv f;
+    f.d = d;
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    f.shift = 31 + s;
+    f.mul = (1ull << f.shift) / d + 1;
+    return f;
+  }
+  __host__ __device__ __forceinline__ uint32_t div(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
+};
+
+inline int type_bytes(int t) { return t == FA_F32 ? 4 : 2; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// kernel(arg) on the stream. hipLaunchKernel returns its own status: an error that an earlier call left behind is not
+// taken for this launch's.
+template <typename P>
+inline void launch(void (*kernel)(P), dim3 grid, dim3 block, size_t lds, hipStream_t s, P arg) {
+  void* args[] = {&arg};
+  FA_HIP(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, args, lds, s));
+}
+
+// compute units of the current device (an attribute query: no allocation, no synchronisation, legal during capture)
+inline int cu_count() {
+  int dev = 0, n = 0;
+  FA_HIP(hipGetDevice(&dev));
+  FA_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
+  return n;
+}
+
+}  // namespace fa

@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/funasr_hip.h"
+#include "api.h"
 #include "common.h"
 #include "gguf.h"
 #include "kernels.h"
@@ -1768,21 +1769,6 @@ using fa::Engine;
 struct fa_engine {
   Engine* e;
 };
-
-#define FA_API_BEGIN try {
-#define FA_API_END                 \
-  }                                \
-  catch (fa::hip_failure&) {       \
-    return FA_ERR_HIP;             \
-  }                                \
-  catch (fa::arg_failure&) {       \
-    return FA_ERR_ARG;             \
-  }                                \
-  catch (std::exception & ex) {    \
-    fa::set_error(ex.what());      \
-    return FA_ERR_STATE;           \
-  }                                \
-  return FA_OK;
 
 extern "C" {
 

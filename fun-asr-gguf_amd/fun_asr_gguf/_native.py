@@ -24,6 +24,8 @@ EXPORTS = [
     "fa_llm_invariant_width", "fa_set_encode_mode", "fa_ctc_head", "fa_set_tensor_u8dq", "fa_set_ctc_int8",
     "fa_ctc_int8_active", "fa_comm_unique_id", "fa_comm_init", "fa_comm_allgather_sizes", "fa_comm_allgather_bytes",
     "fa_comm_destroy", "fa_llm_prefill_rows", "fa_encode_generation", "fa_llm_decode_recoveries",
+    "fa_qk_norm_rope", "fa_kv_append", "fa_tree_attention", "fa_tree_attention_workspace", "fa_sample_tokens",
+    "fa_sample_tokens_workspace",
 ]
 
 
@@ -42,6 +44,38 @@ class LlmConfig(ctypes.Structure):
 class Sampling(ctypes.Structure):
     _fields_ = [("temperature", ctypes.c_float), ("top_p", ctypes.c_float), ("top_k", ctypes.c_int32),
                 ("seed", ctypes.c_uint32)]
+
+
+def _fields(kind, names):
+    return [(n, kind) for n in names.split()]
+
+
+class HeadRowsArgs(ctypes.Structure):
+    """fa_head_rows_args (fa_qk_norm_rope, fa_kv_append)."""
+    _fields_ = (_fields(ctypes.c_void_p, "q k v q_out k_out v_out q_weight k_weight cos sin positions slots") +
+                _fields(ctypes.c_int64, "q_token q_head k_token k_head v_token v_head q_out_token q_out_head k_out_token "
+                                        "k_out_head k_out_page v_out_token v_out_head v_out_page") +
+                _fields(ctypes.c_int32, "tokens heads kv_heads head_dim rot_dim table_len type cache_type positions_64 "
+                                        "slots_64 interleaved pages page_size") +
+                [("eps", ctypes.c_float)])
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """fa_tree_attention_args."""
+    _fields_ = (_fields(ctypes.c_void_p, "q out k_cache v_cache block_table context_lens draft_lens mask workspace") +
+                _fields(ctypes.c_int64, "workspace_bytes q_seq q_node q_head out_seq out_node out_head k_page k_head k_slot "
+                                        "v_page v_head v_slot table_seq mask_seq mask_row") +
+                _fields(ctypes.c_int32, "seqs nodes heads kv_heads head_dim q_type cache_type pages page_size table_len "
+                                        "max_context") +
+                [("scale", ctypes.c_float)])
+
+
+class SampleArgs(ctypes.Structure):
+    """fa_sample_args."""
+    _fields_ = (_fields(ctypes.c_void_p, "logits u temperatures top_ps min_ps top_ks token_out prob_out workspace") +
+                _fields(ctypes.c_int64, "workspace_bytes row_stride") +
+                _fields(ctypes.c_int32, "rows vocab type top_k") +
+                _fields(ctypes.c_float, "temperature top_p min_p"))
 
 
 _lib = None
@@ -118,6 +152,9 @@ def load():
     lib.fa_token_piece.argtypes = [P, I32, ctypes.c_char_p, I32, P]
     lib.fa_gguf_read_tensor.argtypes = [ctypes.c_char_p, ctypes.c_char_p, I32, P, I64]
     lib.fa_fuzzy_substring_distance.argtypes = [P, I32, P, I32, P]
+    for f in ("fa_qk_norm_rope", "fa_kv_append", "fa_tree_attention", "fa_tree_attention_workspace", "fa_sample_tokens",
+              "fa_sample_tokens_workspace"):
+        getattr(lib, f).argtypes = [P, P]
     _lib = lib
     return lib
 

@@ -266,6 +266,104 @@ int fa_profile_enable(fa_engine* e, int32_t on);
 int fa_profile_read(fa_engine* e, int32_t cls, double* ms, int64_t* launches, double* bytes, double* flops);
 int fa_synchronize(fa_engine* e);
 
+/* ---- drafted-token operators on device tensors. What a decoding step that verifies drafted tokens needs beside the
+ * engine's own layers: head norms with the rotation, a paged key / value cache, attention of a tree of drafted tokens over
+ * it, and draws from given random numbers. No engine is involved: every pointer is device memory of the current device,
+ * the work is enqueued on `stream` (a hipStream_t, NULL: the default stream) and nothing is allocated, synchronised or
+ * copied to the host, so every call can be captured into a graph. Workspaces are the caller's: a call owns its workspace
+ * until its work on the stream is done (two calls that may run at the same time need two). Sizes, strides (in elements),
+ * types and alignment are checked before anything is enqueued (FA_ERR_ARG). What only the device knows is guarded there:
+ * see each call. */
+#define FA_F32 0
+#define FA_F16 1
+#define FA_BF16 2
+
+/* Head rows of q, k and v: x [tokens, heads, head_dim], the last dimension contiguous, any other strides.
+ * q and k rows become y = rot(x / sqrt(mean(x^2) + eps) * weight) in 32 bits, rounded once to the output's type;
+ * a NULL weight leaves the norm out, NULL cos / sin the rotation. The rotation turns the pairs (i, i + rot_dim / 2)
+ * (interleaved: (2 i, 2 i + 1)) of the first rot_dim dimensions by the angle whose cosine and sine are cos / sin
+ * [table_len, rot_dim / 2] (rows contiguous) at the token's position; the dimensions behind rot_dim pass through.
+ * head_dim and rot_dim are multiples of 16, head_dim at most 512. A token whose position lies outside the table is
+ * left out: nothing of it is written. An output may be its own input (in place), no other overlap. */
+typedef struct fa_head_rows_args {
+  const void *q, *k, *v;               /* v: fa_kv_append only; q and k may be NULL where their heads are 0 */
+  void *q_out, *k_out, *v_out;         /* k_out / v_out: rows (fa_qk_norm_rope) or caches (fa_kv_append) */
+  const float *q_weight, *k_weight, *cos, *sin;
+  const void *positions, *slots;       /* [tokens] int32 or int64 */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;   /* strides, elements */
+  int64_t q_out_token, q_out_head;
+  int64_t k_out_token, k_out_head, k_out_page;                 /* caches: slot within a page, head, page */
+  int64_t v_out_token, v_out_head, v_out_page;
+  int32_t tokens, heads, kv_heads, head_dim, rot_dim, table_len;
+  int32_t type, cache_type;            /* FA_F32 / FA_F16 / FA_BF16; cache_type: fa_kv_append, FA_F16 / FA_BF16 */
+  int32_t positions_64, slots_64, interleaved;
+  int32_t pages, page_size;            /* fa_kv_append */
+  float eps;
+} fa_head_rows_args;
+/* Norm and rotation of q (heads) and k (kv_heads) rows into q_out / k_out of the same type (the llama.cpp graph's
+ * rms_norm + rope of Qwen3 heads, which the engine's decode kernels fuse for their own shapes). */
+int fa_qk_norm_rope(const fa_head_rows_args* a, void* stream);
+/* The same for k (and q, where heads > 0), with k and v written into a paged cache: k_out / v_out
+ * [pages, kv_heads, page_size, head_dim] (any strides that keep rows 16-byte aligned), token t at slot
+ * slots[t] = page * page_size + offset. A token with a slot outside [0, pages * page_size) (padding: -1) is not appended;
+ * its q row is still made. The slots of one call are distinct: of two tokens with one slot, either's values may stay. */
+int fa_kv_append(const fa_head_rows_args* a, void* stream);
+
+/* Attention of drafted tokens over a paged cache. Sequence b has context_lens[b] committed tokens and, behind them in its
+ * pages, draft_lens[b] drafted ones (NULL: nodes for every sequence), whose keys and values have been appended at the
+ * logical positions context_lens[b] + j. Key position p of sequence b lies in page block_table[b][p / page_size] at
+ * offset p % page_size. Drafted token i sees every committed key and the drafted keys j with mask[b][i][j] != 0
+ * (NULL: j <= i, so nodes = 1 is an ordinary decoding step and a chain is verified or prefilled causally):
+ *   out[b][i] = softmax_j(scale * q[b][i] . k[j]) v[j], statistics in 32 bits; a row that sees no key is 0.
+ * q / out [seqs, nodes, heads, head_dim], head h reads kv head h / (heads / kv_heads). q_type is cache_type, or FA_F32
+ * (then q and the probabilities enter the products as sums of 16-bit terms, which keeps 32-bit accuracy). head_dim is a
+ * multiple of 8, at most 256. Rows of out with i >= draft_lens[b] are left as they were. Lengths are cut to what the
+ * block table holds; a page number outside [0, pages) makes its keys absent. max_context bounds context_lens for the
+ * split of long sequences over the card (a longer one is still computed right, only slower). */
+typedef struct fa_tree_attention_args {
+  const void* q;
+  void* out;
+  const void *k_cache, *v_cache;       /* [pages, kv_heads, page_size, head_dim] */
+  const int32_t *block_table, *context_lens, *draft_lens;
+  const uint8_t* mask;                 /* [seqs, nodes, nodes] bytes, strides below (0: shared by the sequences) */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_seq, q_node, q_head, out_seq, out_node, out_head;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  int64_t table_seq, mask_seq, mask_row;
+  int32_t seqs, nodes, heads, kv_heads, head_dim;
+  int32_t q_type, cache_type, pages, page_size, table_len, max_context;
+  float scale;
+} fa_tree_attention_args;
+/* Bytes of workspace the call needs (0: none); depends on the sizes, types and max_context alone. */
+int fa_tree_attention_workspace(const fa_tree_attention_args* a, int64_t* bytes);
+int fa_tree_attention(const fa_tree_attention_args* a, void* stream);
+
+/* One token for every row of logits [rows, vocab], from a given random number u[row] in [0, 1): the sampler chain
+ * top_k -> top_p (min_keep 1, softmax at temperature 1 over the top_k) -> min_p (p >= min_p * max p) -> temperature, then
+ * the first token i, in the vocabulary's order, whose cumulative mass exceeds u * total. Equal logits: the lower id ranks
+ * higher. temperature <= 0: the largest logit. top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 switch a step off. NaN
+ * logits count as -inf; a row with nothing above -inf gives token -1 and probability 0; +inf logits share the whole mass.
+ * Sums are exact integers (weights rounded to 2^-44 of the largest at a vocabulary of 2^18), so a result depends on the
+ * row alone. Settings: the scalars, or per-row device arrays where not NULL. prob_out (nullable): the token's
+ * probability. fa_sampling's chain draws from its own counters; this one is for callers that bring the random numbers
+ * (speculative verification, reproducible serving). */
+typedef struct fa_sample_args {
+  const void* logits;
+  const float* u;
+  const float *temperatures, *top_ps, *min_ps;
+  const int32_t* top_ks;
+  int32_t* token_out;
+  float* prob_out;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t row_stride;
+  int32_t rows, vocab, type, top_k;
+  float temperature, top_p, min_p;
+} fa_sample_args;
+int fa_sample_tokens_workspace(const fa_sample_args* a, int64_t* bytes);
+int fa_sample_tokens(const fa_sample_args* a, void* stream);
+
 /* ---- result gather over RCCL (the reference decodes segments sequentially, orchestrator.py:139-171,
  * so this is the only exchange of the sharded path): one communicator per engine. Rank 0 creates a 128-byte id, the
  * caller hands it to every rank by any side channel, each rank joins with fa_comm_init. The gather is two all-gathers
