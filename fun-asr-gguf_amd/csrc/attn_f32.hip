@@ -21,7 +21,10 @@
 namespace fa {
 
 // fp16 encoder mode (C5): the attention output (an fp16 tensor in the float16 graph) rounded to fp16
+// (the values are pinned as f32 first: folded into the multiply before it, v_fma_mixlo_f16, a product would be rounded once
+// in some instantiations and twice in others)
 __device__ __forceinline__ float4 round_f16x4(float4 v) {
+  asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
   return make_float4(__half2float(__float2half_rn(v.x)), __half2float(__float2half_rn(v.y)),
                      __half2float(__float2half_rn(v.z)), __half2float(__float2half_rn(v.w)));
 }

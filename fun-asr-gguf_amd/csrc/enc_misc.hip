@@ -142,10 +142,11 @@ __global__ void k_layernorm(const float* __restrict__ x, int64_t ldx, float* __r
     for (int i = 0; i < PER; i += 4) {
       const int c = lane * PER + i;
       const float4 wv = *reinterpret_cast<const float4*>(w + c), bv = *reinterpret_cast<const float4*>(bb + c);
-      o[i / 4] = make_float4(r16e((v[i] - mean) * rstd * wv.x + bv.x, r16) * mk,
-                             r16e((v[i + 1] - mean) * rstd * wv.y + bv.y, r16) * mk,
-                             r16e((v[i + 2] - mean) * rstd * wv.z + bv.z, r16) * mk,
-                             r16e((v[i + 3] - mean) * rstd * wv.w + bv.w, r16) * mk);
+      float4 f = make_float4((v[i] - mean) * rstd * wv.x + bv.x, (v[i + 1] - mean) * rstd * wv.y + bv.y,
+                             (v[i + 2] - mean) * rstd * wv.z + bv.z, (v[i + 3] - mean) * rstd * wv.w + bv.w);
+      // pinned as f32: the fp16 graph's rounding must not fold into the multiply-add (v_fma_mixlo_f16 rounds once)
+      asm volatile("" : "+v"(f.x), "+v"(f.y), "+v"(f.z), "+v"(f.w));
+      o[i / 4] = make_float4(r16e(f.x, r16) * mk, r16e(f.y, r16) * mk, r16e(f.z, r16) * mk, r16e(f.w, r16) * mk);
       if (!yp.hi) *reinterpret_cast<float4*>(y + yo + c) = o[i / 4];
     }
     if (yp.hi) {  // bf16x3 consumer only: the planes its staging would form from these f32 values, 16 B per store
