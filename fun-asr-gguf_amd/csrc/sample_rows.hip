@@ -2,34 +2,90 @@
 //
 // The chain keeps a set of tokens that is always a prefix of the order (logit descending, id ascending): top_k a prefix of k,
 // top_p the shortest prefix whose softmax mass reaches p of the top_k's, min_p a bound on the logit. So the set is held as a
-// cut (key of the last logit kept, last id kept among its equals), nothing is sorted but a few thousand values near a cut,
-// and the draw runs through the vocabulary in its own order.
+// cut (key of the last logit kept, last id kept among its equals), nothing is sorted but the few values near a cut, and the
+// draw runs through the vocabulary in its own order.
 //
 // Weights exp(x - max) are rounded to integers of 2^-S of the largest (S = 62 - ceil(log2 vocab)), so that sums are exact
 // whatever the order in which they are added: results do not depend on the launch shape or on atomics. The exponentials are
 // taken in 64 bits, because a sum over 150 000 tokens is compared with borders 7e-6 apart.
+//
+// A row is cut into chunks of 16 values a thread, one block each, so that a single row still uses many compute units:
+//   k_scan    the chunk's maximum; with a small top_k also every thread's maximum.
+//   k_select  rows with a top_k up to KMAX: one block finishes the row. The k largest lie in the groups of 16 whose maximum is
+//             in the bins that hold k such maxima, so only those groups are read again (a few hundred values).
+//             rows with a top_p or a larger top_k: a histogram (count and mass by steps of 1/32 below the maximum); the block
+//             that arrives last finds the bins in which the cuts lie.
+//   k_draw    the other rows: each chunk's mass at the temperature, the values in the cuts' bins to a list; the block that
+//             arrives last sorts the list, fixes the cut, picks the chunk and the token in it.
+// Nothing waits for another block. A row whose cut's bins hold more than CAP values (thousands of equal logits) is finished
+// by one block that narrows the cut by key instead (general_row).
 #include "api.h"
 #include "draft_ops.h"
 
+#include <algorithm>
+
 namespace fa {
 
-constexpr int ST = 1024, SW = ST / 64;  // threads, waves
-constexpr int BINS = 1024;              // of 1 / 32 below the maximum; the last takes everything 32 and more below
-constexpr int CAP = 4096;               // values that are sorted
+constexpr int PER = 16;     // values a thread
+constexpr int BINS = 1024;  // of 1 / 32 below the maximum; the last takes everything 32 and more below
+constexpr int CAP = 4096;   // values that are sorted
+constexpr int ST = 1024;    // threads of k_select
+constexpr int KMAX = 1024;  // largest top_k that k_select finishes itself
+
+typedef unsigned long long u64;
+
+struct RowState {  // zeroed by k_scan
+  uint32_t arrived_select, arrived_draw, list_n, overflow;
+  int b_lo, b_hi, b_k, pad;  // bins of the cut: the listed ones are [b_lo, b_hi] and b_k
+  u64 mass_lo, mass_k;       // mass before b_lo / before b_k
+  u64 cnt_k;                 // values before b_k
+  u64 total;                 // mass of the row
+};
 
 struct SampleP {
   fa_sample_args a;
   double one;  // 2^S
+  int chunks;           // of PER values a thread of k_scan and k_draw
+  int sel_chunks;       // of k_select, whose blocks have ST threads whatever the others' have
+  FastDiv grid_div;     // blocks a row in this launch (1 where the first alone has work)
+  int grid_chunks;
+  int want_max;  // the threads' maxima are wanted (a row may have a small top_k)
+  float* cmax;   // [rows][chunks]
+  int* cidx;
+  u64* cmass;
+  u64* hist_mass;  // [rows][BINS]
+  uint32_t* hist_cnt;
+  u64* list;  // [rows][CAP]
+  RowState* state;
+  float* tmax;  // [rows][chunks][threads]
 };
 
+enum RowKind { GREEDY, SMALL_K, HIST, PLAIN };
 struct RowSettings {
-  float temperature, top_p, min_p;
+  float top_p;
+  double inv_t, least;  // 1 / temperature; least logit above the maximum (min_p)
   int top_k;
+  bool has_k, has_p;
+  RowKind kind;
 };
+__device__ __forceinline__ RowSettings settings_of(const fa_sample_args& a, int r) {
+  RowSettings s;
+  const float t = a.temperatures ? a.temperatures[r] : a.temperature, m = a.min_ps ? a.min_ps[r] : a.min_p;
+  s.top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+  s.top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+  s.has_k = s.top_k > 0 && s.top_k < a.vocab;
+  s.has_p = s.top_p < 1.f;
+  s.inv_t = 1.0 / (double)t;
+  s.least = m > 0.f ? ::log((double)m) : -INFINITY;
+  s.kind = !(t > 0.f) || s.top_k == 1 || !(s.top_p > 0.f) || !(m <= 1.f) ? GREEDY
+           : s.has_k && s.top_k <= KMAX                                    ? SMALL_K
+           : s.has_k || s.has_p                                            ? HIST
+                                                                           : PLAIN;
+  return s;
+}
 
-template <typename T>
-__device__ __forceinline__ float logit(const T* row, int i) {  // NaN -> -inf, -0 -> 0
-  const float x = (float)row[i] + 0.0f;
+__device__ __forceinline__ float clean(float x) {  // NaN -> -inf, -0 -> 0
+  x += 0.0f;
   return x != x ? -INFINITY : x;
 }
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -37,14 +93,32 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
+// monotone in x; a maximum of inf: everything else in the last bin
 __device__ __forceinline__ int bin_of(float x, float top) {
-  return x == top ? 0 : (int)fminf((top - x) * 32.f, (float)(BINS - 1));  // monotone in x; top = inf: the last bin
+  return x == top ? 0 : (int)fminf((top - x) * 32.f, (float)(BINS - 1));
 }
 __device__ __forceinline__ double rel_of(float x, float top) { return x == top ? 0.0 : (double)x - (double)top; }
-__device__ __forceinline__ unsigned long long weight(double rel, double one) {
-  return (unsigned long long)(exp(rel) * one + 0.5);  // exp(-inf) = 0
+// exp(x) 2^S, rounded, for x <= 0: x = n ln 2 + 4 r with |r| <= ln 2 / 8, the Taylor polynomial of degree 9 in r
+// (remainder r^10 / 10! < 7e-18 of 1), squared twice: relative error below 4e-15 before the rounding to an integer
+__device__ __forceinline__ u64 weight(double x, double one) {
+  if (!(x > -60.0)) return 0;  // 2^62 exp(-60) < 1/2 (NaN: -inf times 1 / inf)
+  const double n = rint(x * 1.4426950408889634);
+  double r = fma(n, -0x1.62e42fefa39efp-1, x);
+  r = fma(n, -0x1.abc9e3b39803fp-56, r) * 0.25;
+  double p = 1.0 / 362880.0;
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  p *= p;
+  p *= p;
+  return (u64)(ldexp(p, (int)n) * one + 0.5);
 }
-__device__ __forceinline__ unsigned long long shfl_xor64(unsigned long long v, int o) { return __shfl_xor(v, o); }
 
 struct Cut {  // the last value kept
   uint32_t key;
@@ -54,39 +128,151 @@ __device__ __forceinline__ bool within(uint32_t key, int i, const Cut& c) {
   return key > c.key || (key == c.key && i <= c.idx);
 }
 
+// A chunk's values: thread t holds index base + (j * BT + t) * W + w as value j * W + w, W = 16 bytes' worth where the row is
+// 16-byte aligned, else 1: coalesced either way, and index order within each j
+template <typename T>
+struct RowView {
+  const T* p;
+  int V;
+  bool vec;
+};
+template <typename T>
+__device__ __forceinline__ RowView<T> row_view(const fa_sample_args& a, int r) {
+  RowView<T> v;
+  v.p = reinterpret_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
+  v.V = a.vocab;
+  v.vec = (reinterpret_cast<uintptr_t>(v.p) & 15) == 0;
+  return v;
+}
+template <typename T> constexpr int kWide = 16 / (int)sizeof(T);
+template <typename T, int BT>
+__device__ __forceinline__ int index_at(bool vec, int base, int t, int e) {
+  constexpr int W = kWide<T>;
+  return vec ? base + ((e / W) * BT + t) * W + e % W : base + e * BT + t;
+}
+template <typename T, int BT>
+__device__ __forceinline__ void load_chunk(const RowView<T>& v, int base, int t, float (&x)[PER]) {
+  constexpr int W = kWide<T>;
+  if (v.vec) {
+#pragma unroll
+    for (int j = 0; j < PER / W; ++j) {
+      const int i = base + (j * BT + t) * W;
+      T y[W];
+      if (i + W <= v.V) {
+        *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(v.p + i);
+#pragma unroll
+        for (int w = 0; w < W; ++w) x[j * W + w] = clean((float)y[w]);
+      } else {
+#pragma unroll
+        for (int w = 0; w < W; ++w) x[j * W + w] = i + w < v.V ? clean((float)v.p[i + w]) : -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int i = base + e * BT + t;
+      x[e] = i < v.V ? clean((float)v.p[i]) : -INFINITY;
+    }
+  }
+}
+
+__device__ __forceinline__ u64 wave_sum64(u64 v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  return v;
+}
+__device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const u64 u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ int first_lane(uint64_t m) { return __ffsll((unsigned long long)m) - 1; }
+
+// values that blocks of one launch hand to each other pass the per-XCD caches: relaxed device-scope accesses
+template <typename X>
+__device__ __forceinline__ X dev_load(const X* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename X>
+__device__ __forceinline__ void dev_store(X* p, X v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename X>
+__device__ __forceinline__ X dev_add(X* p, X v) {
+  return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <int BT>
 struct Shared {
-  unsigned long long mass[BINS];
+  u64 mass[BINS];
   uint32_t cnt[BINS];
-  unsigned long long list[CAP];
-  unsigned long long wsum[SW];
-  float wmax[SW];
-  int widx[SW], wcnt[SW];
-  uint32_t wlo[SW], whi[SW];
-  int n, sel;
-  unsigned long long before_mass, mass_sel;
+  u64 list[CAP];
+  u64 part[PER * BT / 64];
+  float wmax[BT / 64];
+  int widx[BT / 64], wcnt[BT / 64];
+  uint32_t wlo[BT / 64], whi[BT / 64];
+  int n, sel, flag, pick;
+  u64 before_mass, mass_sel, total, chunk_before;
   uint32_t before_cnt;
   Cut cut;
-  int token;
-  float prob;
 };
 
-// first bin at which the running count reaches `need` (count) or the running mass reaches `target` -> S.sel, with what lies
-// before it in S.before_*; -1: none. Wave 0, 16 bins a lane.
-__device__ __forceinline__ void find_bin(Shared& S, bool by_mass, uint32_t need, double target, uint32_t c0,
-                                         unsigned long long m0) {
+// true in the block that is the last of `n` to come here (block-uniform). Everything the block has handed over lies before
+template <int BT>
+__device__ __forceinline__ bool last_to_arrive(Shared<BT>& S, uint32_t* counter, int n) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) S.flag = dev_add(counter, 1u) == (uint32_t)n - 1;
+  __syncthreads();
+  return S.flag != 0;
+}
+
+// the row's largest value and its lowest index, from the chunks' -> every thread
+template <int BT>
+__device__ __forceinline__ float row_top(Shared<BT>& S, const SampleP& P, int r, int& at) {
+  const int lane = threadIdx.x & 63;
+  float top = -INFINITY;
+  at = 0x7FFFFFFF;
+  for (int c = lane; c < P.chunks; c += 64) {  // every wave for itself: no barrier
+    const float x = P.cmax[(int64_t)r * P.chunks + c];
+    if (x > top) {
+      top = x;
+      at = P.cidx[(int64_t)r * P.chunks + c];
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const float x = __shfl_xor(top, o);
+    const int j = __shfl_xor(at, o);
+    if (x > top || (x == top && j < at)) {
+      top = x;
+      at = j;
+    }
+  }
+  return top;
+}
+
+// first bin at which the running count reaches `need` or, by mass, the running mass reaches `target` -> S.sel, with what
+// lies before it in S.before_*; -1: none. Wave 0, 16 bins a lane. Ends with a barrier.
+template <int BT>
+__device__ __forceinline__ void find_bin(Shared<BT>& S, bool by_mass, uint32_t need, double target, uint32_t c0, u64 m0) {
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
-    uint32_t c = 0;
-    unsigned long long m = 0;
+    uint32_t c = 0, ci;
+    u64 m = 0, mi;
+#pragma unroll
     for (int i = 0; i < BINS / 64; ++i) {
       c += S.cnt[lane * (BINS / 64) + i];
       m += S.mass[lane * (BINS / 64) + i];
     }
-    uint32_t ci = c;
-    unsigned long long mi = m;
+    ci = c;
+    mi = m;
     for (int o = 1; o < 64; o <<= 1) {
       const uint32_t cu = __shfl_up(ci, o);
-      const unsigned long long mu = __shfl_up(mi, o);
+      const u64 mu = __shfl_up(mi, o);
       if (lane >= o) {
         ci += cu;
         mi += mu;
@@ -94,15 +280,16 @@ __device__ __forceinline__ void find_bin(Shared& S, bool by_mass, uint32_t need,
     }
     const bool reached = by_mass ? (double)(m0 + mi) >= target : c0 + ci >= need;
     const uint64_t who = __ballot(reached);
+    if (lane == 63) S.total = m0 + mi;
     if (who == 0) {
       if (lane == 0) S.sel = -1;
-    } else if (lane == __ffsll((unsigned long long)who) - 1) {
+    } else if (lane == first_lane(who)) {
       uint32_t cb = c0 + ci - c;
-      unsigned long long mb = m0 + mi - m;
+      u64 mb = m0 + mi - m;
       int i = lane * (BINS / 64);
       for (;; ++i) {
         const uint32_t cn = cb + S.cnt[i];
-        const unsigned long long mn = mb + S.mass[i];
+        const u64 mn = mb + S.mass[i];
         if (by_mass ? (double)mn >= target : cn >= need) break;
         cb = cn;
         mb = mn;
@@ -115,66 +302,92 @@ __device__ __forceinline__ void find_bin(Shared& S, bool by_mass, uint32_t need,
   __syncthreads();
 }
 
-template <typename T>
-__global__ __launch_bounds__(ST) void k_sample_row(SampleP P) {
-  __shared__ Shared S;
-  const fa_sample_args& a = P.a;
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab;
-  const T* const row = reinterpret_cast<const T*>(a.logits) + (int64_t)r * a.row_stride;
-  RowSettings s;
-  s.temperature = a.temperatures ? a.temperatures[r] : a.temperature;
-  s.top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-  s.min_p = a.min_ps ? a.min_ps[r] : a.min_p;
-  s.top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-
-  // the largest logit, its lowest id
-  float top = -INFINITY;
-  int at = 0x7FFFFFFF;
-  for (int i = tid; i < V; i += ST) {
-    const float x = logit(row, i);
-    if (x > top) {
-      top = x;
-      at = i;
+// S.list[0 .. n) ascending; every entry is unique. A few hundred: each finds its own rank; more: bitonic
+template <int BT>
+__device__ __forceinline__ void sort_list(Shared<BT>& S, int n) {
+  const int tid = threadIdx.x;
+  if (n <= 256 && n <= BT) {
+    u64 mine = 0;
+    int rank = 0;
+    if (tid < n) {
+      mine = S.list[tid];
+      for (int i = 0; i < n; ++i) rank += S.list[i] < mine;
     }
-  }
-  for (int o = 1; o < 64; o <<= 1) {
-    const float x = __shfl_xor(top, o);
-    const int j = __shfl_xor(at, o);
-    if (x > top || (x == top && j < at)) {
-      top = x;
-      at = j;
-    }
-  }
-  if (lane == 0) {
-    S.wmax[wave] = top;
-    S.widx[wave] = at;
-  }
-  __syncthreads();
-  for (int w = 0; w < SW; ++w)
-    if (S.wmax[w] > top || (S.wmax[w] == top && S.widx[w] < at)) {
-      top = S.wmax[w];
-      at = S.widx[w];
-    }
-  const bool greedy = !(s.temperature > 0.f) || s.top_k == 1 || !(s.top_p > 0.f) || !(s.min_p <= 1.f);
-  if (top == -INFINITY || greedy) {
-    if (tid == 0) {
-      a.token_out[r] = top == -INFINITY ? -1 : at;
-      if (a.prob_out) a.prob_out[r] = top == -INFINITY ? 0.f : 1.f;
-    }
+    __syncthreads();
+    if (tid < n) S.list[rank] = mine;
+    __syncthreads();
     return;
   }
-  const bool has_k = s.top_k > 0 && s.top_k < V, has_p = s.top_p < 1.f;
-  const double least = s.min_p > 0.f ? ::log((double)s.min_p) : -INFINITY;
+  int m = 64;
+  while (m < n) m *= 2;
+  for (int i = n + tid; i < m; i += BT) S.list[i] = ~0ull;
+  __syncthreads();
+  for (int k = 2; k <= m; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = tid; i < m; i += BT) {
+        const int o = i ^ j;
+        if (o > i) {
+          const u64 x = S.list[i], y = S.list[o];
+          if ((x > y) == ((i & k) == 0)) {
+            S.list[i] = y;
+            S.list[o] = x;
+          }
+        }
+      }
+      __syncthreads();
+    }
+}
+__device__ __forceinline__ u64 entry_of(float x, int i) { return ((u64)(~order_key(x)) << 32) | (uint32_t)i; }
+__device__ __forceinline__ uint32_t entry_key(u64 e) { return ~(uint32_t)(e >> 32); }
+
+// the first of the sorted list's values [i0, n) at which the mass, m0 lying before i0, reaches `target` -> its place, and the
+// mass up to and with it; -1: none. Every wave alike.
+template <int BT>
+__device__ __forceinline__ int list_reach(const Shared<BT>& S, int i0, int n, double target, u64 m0, float top, double one,
+                                          u64& mass) {
+  const int lane = threadIdx.x & 63;
+  for (int i = i0; i < n; i += 64) {
+    const u64 w = i + lane < n ? weight(rel_of(key_value(entry_key(S.list[i + lane])), top), one) : 0;
+    const u64 mi = m0 + wave_scan64(w, lane);
+    const uint64_t who = __ballot(i + lane < n && (double)mi >= target);
+    if (who) {
+      const int l = first_lane(who);
+      mass = __shfl(mi, l);
+      return i + l;
+    }
+    m0 = __shfl(mi, 63);
+  }
+  mass = m0;
+  return -1;
+}
+
+// Where a draw of `total` lies: u total, at or past the end for u >= 1 (then the last token kept is taken)
+__device__ __forceinline__ double draw_target(float u, u64 total) { return (u > 0.f ? (double)u : 0.0) * (double)total; }
+
+__device__ __forceinline__ void put(const SampleP& P, int r, int token, u64 w, u64 total) {
+  P.a.token_out[r] = token;
+  if (P.a.prob_out) P.a.prob_out[r] = (float)((double)w / (double)total);
+}
+
+// ------------------------------------------------------------------------------------------------------------ general row
+// One block finishes a row by narrowing the cut in the keys' space: no list that could overflow, many passes over the row.
+template <typename T, int BT>
+__device__ __forceinline__ void general_row(Shared<BT>& S, const SampleP& P, int r, float top) {
+  constexpr int NW = BT / 64;
+  const fa_sample_args& a = P.a;
+  const RowSettings s = settings_of(a, r);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab;
+  const T* const row = row_view<T>(a, r).p;
+  auto logit = [&](int i) { return clean((float)row[i]); };
   Cut cut{0, 0x7FFFFFFF};  // everything
 
   // narrows the cut inside bin b: the prefix of the bin's values (of those within `lim`) at which the count reaches `need`, or
   // the mass `target`, c0 / m0 lying before the bin -> S.cut, S.mass_sel (mass up to the cut)
-  auto resolve = [&](int b, const Cut lim, bool by_mass, uint32_t need, double target, uint32_t c0,
-                     unsigned long long m0) {
+  auto resolve = [&](int b, const Cut lim, bool by_mass, uint32_t need, double target, uint32_t c0, u64 m0) {
     uint32_t lo = 0, hi = 0xFFFFFFFFu;
     auto each = [&](auto f) {
-      for (int i = tid; i < V; i += ST) {
-        const float x = logit(row, i);
+      for (int i = tid; i < V; i += BT) {
+        const float x = logit(i);
         if (x == -INFINITY || bin_of(x, top) != b) continue;
         const uint32_t k = order_key(x);
         if (k < lo || k > hi || !within(k, i, lim)) continue;
@@ -204,7 +417,7 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleP P) {
       if (tid == 0) S.n = 0;
       __syncthreads();
       n = 0;
-      for (int w = 0; w < SW; ++w) {
+      for (int w = 0; w < NW; ++w) {
         mn = min(mn, S.wlo[w]);
         mx = max(mx, S.whi[w]);
         n += S.wcnt[w];
@@ -213,7 +426,7 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleP P) {
       hi = mx;
       if (n <= CAP) break;
       if (lo == hi) {  // equal values: so many of them, in the order of their ids
-        const unsigned long long w = weight(rel_of(key_value(lo), top), P.one);
+        const u64 w = weight(rel_of(key_value(lo), top), P.one);
         uint32_t c = need - c0;
         if (by_mass) {
           const double f = ceil((target - (double)m0) / (double)w);
@@ -221,9 +434,9 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleP P) {
           while (c > 1 && (double)(m0 + (c - 1) * w) >= target) --c;
           while (c < (uint32_t)n && (double)(m0 + c * w) < target) ++c;
         }
-        const int seg = (V + SW - 1) / SW, i0 = wave * seg, i1 = min(V, i0 + seg);
+        const int seg = (V + NW - 1) / NW, i0 = wave * seg, i1 = min(V, i0 + seg);
         int mine = 0;
-        for (int i = i0 + lane; i < i1; i += 64) mine += order_key(logit(row, i)) == lo;
+        for (int i = i0 + lane; i < i1; i += 64) mine += order_key(logit(i)) == lo;
         mine = wave_sum_i(mine);
         if (lane == 0) S.widx[wave] = mine;
         __syncthreads();
@@ -231,7 +444,7 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleP P) {
         for (int x = 0; x < wave; ++x) before += S.widx[x];
         if (before < (int)c && before + mine >= (int)c) {
           for (int i = i0; i < i1; i += 64) {
-            const bool is = i + lane < i1 && order_key(logit(row, i + lane)) == lo;
+            const bool is = i + lane < i1 && order_key(logit(i + lane)) == lo;
             const uint64_t who = __ballot(is);
             const int here = __popcll(who);
             if (before + here >= (int)c) {
@@ -246,10 +459,10 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleP P) {
         __syncthreads();
         return;
       }
-      // 1024 equal steps of the key's range, downwards
+      // 1024 equal steps of the keys' range, downwards
       int sh = 0;
       while (((hi - lo) >> sh) >= BINS) ++sh;
-      for (int i = tid; i < BINS; i += ST) {
+      for (int i = tid; i < BINS; i += BT) {
         S.cnt[i] = 0;
         S.mass[i] = 0;
       }
@@ -257,7 +470,7 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleP P) {
       each([&](float x, uint32_t k, int) {
         const int q = (int)((hi - k) >> sh);
         atomicAdd(&S.cnt[q], 1u);
-        if (has_p) atomicAdd(&S.mass[q], weight(rel_of(x, top), P.one));
+        if (s.has_p) atomicAdd(&S.mass[q], weight(rel_of(x, top), P.one));
       });
       __syncthreads();
       find_bin(S, by_mass, need, target, c0, m0);
@@ -269,184 +482,591 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleP P) {
       hi = top_key;
       __syncthreads();
     }
-    // few values: sorted, largest first, lower ids first among equals
-    each([&](float, uint32_t k, int i) {
-      const int j = atomicAdd(&S.n, 1);
-      S.list[j] = ((unsigned long long)(~k) << 32) | (uint32_t)i;
-    });
+    each([&](float x, uint32_t, int i) { S.list[atomicAdd(&S.n, 1)] = entry_of(x, i); });
     __syncthreads();
     const int n = S.n;
-    int m = 64;
-    while (m < n) m *= 2;
-    for (int i = n + tid; i < m; i += ST) S.list[i] = ~0ull;
-    __syncthreads();
-    for (int k = 2; k <= m; k <<= 1)
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        for (int i = tid; i < m; i += ST) {
-          const int o = i ^ j;
-          if (o > i) {
-            const unsigned long long x = S.list[i], y = S.list[o];
-            if ((x > y) == ((i & k) == 0)) {
-              S.list[i] = y;
-              S.list[o] = x;
-            }
-          }
-        }
-        __syncthreads();
-      }
-    if (wave == 0) {
-      for (int i0 = 0; i0 < n; i0 += 64) {
-        const int i = i0 + lane;
-        const unsigned long long e = i < n ? S.list[i] : 0;
-        const uint32_t key = ~(uint32_t)(e >> 32);
-        const unsigned long long w = i < n && has_p ? weight(rel_of(key_value(key), top), P.one) : 0;
-        unsigned long long mi = w;
-        for (int o = 1; o < 64; o <<= 1) {
-          const unsigned long long u = __shfl_up(mi, o);
-          if (lane >= o) mi += u;
-        }
-        const bool reached = i < n && (by_mass ? (double)(m0 + mi) >= target : c0 + i + 1 >= need);
-        const uint64_t who = __ballot(reached);
-        if (who) {
-          if (lane == __ffsll((unsigned long long)who) - 1) {
-            S.cut = Cut{key, (int)(uint32_t)e};
-            S.mass_sel = m0 + mi;
-          }
-          break;
-        }
-        m0 += __shfl(mi, 63);
-      }
+    sort_list(S, n);
+    u64 mass = 0;
+    int at = (int)(need - c0) - 1;
+    if (by_mass) at = list_reach(S, 0, n, target, m0, top, P.one, mass);
+    else if (s.has_p) (void)list_reach(S, 0, at + 1, INFINITY, m0, top, P.one, mass);
+    if (tid == 0) {
+      S.cut = Cut{entry_key(S.list[at]), (int)(uint32_t)S.list[at]};
+      S.mass_sel = mass;
     }
     __syncthreads();
   };
 
-  if (has_k || has_p) {
-    for (int i = tid; i < BINS; i += ST) {
-      S.cnt[i] = 0;
-      S.mass[i] = 0;
-    }
-    __syncthreads();
-    for (int i = tid; i < V; i += ST) {
-      const float x = logit(row, i);
-      if (x == -INFINITY) continue;
-      const int b = bin_of(x, top);
-      atomicAdd(&S.cnt[b], 1u);
-      if (has_p) atomicAdd(&S.mass[b], weight(rel_of(x, top), P.one));
-    }
-    __syncthreads();
-    unsigned long long total = 0;
-    for (int i = 0; i < BINS; ++i) total += S.mass[i];
-    int b = -1;
-    // (the histogram of the row stays in registers over resolve(), which uses its arrays: one bin a thread)
-    const unsigned long long my_mass = S.mass[tid];
-    const uint32_t my_cnt = S.cnt[tid];
-    if (has_k) {
+  if (s.has_k || s.has_p) {
+    auto histogram = [&]() {  // of the values within the cut
+      __syncthreads();
+      for (int i = tid; i < BINS; i += BT) {
+        S.cnt[i] = 0;
+        S.mass[i] = 0;
+      }
+      __syncthreads();
+      for (int i = tid; i < V; i += BT) {
+        const float x = logit(i);
+        if (x == -INFINITY || !within(order_key(x), i, cut)) continue;
+        const int b = bin_of(x, top);
+        atomicAdd(&S.cnt[b], 1u);
+        if (s.has_p) atomicAdd(&S.mass[b], weight(rel_of(x, top), P.one));
+      }
+      __syncthreads();
+    };
+    if (s.has_k) {
+      histogram();
       find_bin(S, false, (uint32_t)s.top_k, 0.0, 0, 0);
-      b = S.sel;
+      const int b = S.sel;
       if (b >= 0) {
         const uint32_t c0 = S.before_cnt;
-        const unsigned long long m0 = S.before_mass;
+        const u64 m0 = S.before_mass;
         resolve(b, cut, false, (uint32_t)s.top_k, 0.0, c0, m0);
         cut = S.cut;
-        total = S.mass_sel;
       }
     }
-    if (has_p) {
-      // the row's histogram again, the last kept bin with what the cut leaves of it
+    if (s.has_p) {
+      histogram();
+      find_bin(S, true, 0, INFINITY, 0, 0);  // the total
+      const double target = (double)s.top_p * (double)S.total;
       __syncthreads();
-      unsigned long long below = 0;
-      S.mass[tid] = my_mass;
-      S.cnt[tid] = my_cnt;
-      __syncthreads();
-      if (b >= 0 && tid == 0) {
-        for (int i = 0; i < b; ++i) below += S.mass[i];
-        S.mass[b] = total - below;
-        for (int i = b + 1; i < BINS; ++i) S.mass[i] = 0;
-      }
-      __syncthreads();
-      const double target = (double)s.top_p * (double)total;
       find_bin(S, true, 0, target, 0, 0);
-      const int bp = S.sel;
-      if (bp >= 0) {
-        const unsigned long long m0 = S.before_mass;
-        resolve(bp, cut, true, 0, target, 0, m0);
-        cut = S.cut;
-      }
+      const int b = S.sel;
+      const u64 m0 = S.before_mass;
+      resolve(b, cut, true, 0, target, 0, m0);
+      cut = S.cut;
     }
   }
 
   // the draw: every wave a run of the row, in order
-  const double inv_t = 1.0 / (double)s.temperature;
-  auto mass_at = [&](int i) -> unsigned long long {
-    const float x = logit(row, i);
+  auto mass_at = [&](int i) -> u64 {
+    const float x = logit(i);
     if (x == -INFINITY || !within(order_key(x), i, cut)) return 0;
     const double rel = rel_of(x, top);
-    return rel < least || rel == -INFINITY ? 0 : weight(rel * inv_t, P.one);
+    return rel < s.least ? 0 : weight(rel * s.inv_t, P.one);
   };
-  const int seg = ((V + SW - 1) / SW + 63) / 64 * 64, i0 = min(V, wave * seg), i1 = min(V, i0 + seg);
-  unsigned long long sum = 0;
+  const int seg = ((V + NW - 1) / NW + 63) / 64 * 64, i0 = min(V, wave * seg), i1 = min(V, i0 + seg);
+  u64 sum = 0;
   for (int i = i0 + lane; i < i1; i += 64) sum += mass_at(i);
-  for (int o = 1; o < 64; o <<= 1) sum += shfl_xor64(sum, o);
+  sum = wave_sum64(sum);
   __syncthreads();
-  if (lane == 0) S.wsum[wave] = sum;
+  if (lane == 0) S.part[wave] = sum;
   __syncthreads();
-  unsigned long long total = 0, before = 0;
+  u64 total = 0, before = 0;
   int last = 0;
-  for (int w = 0; w < SW; ++w) {
-    if (w < wave) before += S.wsum[w];
-    total += S.wsum[w];
-    if (S.wsum[w]) last = w;
+  for (int w = 0; w < NW; ++w) {
+    if (w < wave) before += S.part[w];
+    total += S.part[w];
+    if (S.part[w]) last = w;
   }
-  const float u = a.u[r];
-  const double target = (u > 0.f ? (double)u : 0.0) * (double)total;
-  const bool past = !((double)total > target);  // u >= 1: the last token kept
+  const double target = draw_target(a.u[r], total);
+  const bool past = !((double)total > target);
   const bool mine = past ? wave == last : sum && (double)before <= target && (double)(before + sum) > target;
   if (mine) {
     int tok = -1;
-    unsigned long long wt = 0;
+    u64 wt = 0;
     for (int i = i0; i < i1; i += 64) {
-      const unsigned long long w = i + lane < i1 ? mass_at(i + lane) : 0;
-      unsigned long long mi = w;
-      for (int o = 1; o < 64; o <<= 1) {
-        const unsigned long long x = __shfl_up(mi, o);
-        if (lane >= o) mi += x;
-      }
-      const uint64_t who = __ballot(past ? w != 0 : (double)(before + mi) > target);
-      before += __shfl(mi, 63);
+      const u64 w = i + lane < i1 ? mass_at(i + lane) : 0;
+      const u64 mi = before + wave_scan64(w, lane);
+      const uint64_t who = __ballot(past ? w != 0 : (double)mi > target);
+      before = __shfl(mi, 63);
       if (!who) continue;
-      const int l = past ? 63 - __clzll((long long)who) : __ffsll((unsigned long long)who) - 1;
+      const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
       tok = i + l;
       wt = __shfl(w, l);
       if (!past) break;
     }
-    if (lane == 0) {
-      a.token_out[r] = tok;
-      if (a.prob_out) a.prob_out[r] = (float)((double)wt / (double)total);
-    }
+    if (lane == 0) put(P, r, tok, wt, total);
   }
 }
 
-static SampleP sample_plan(const fa_sample_args* ap) {
-  FA_REQUIRE(ap, "sample_tokens: no arguments");
+// ------------------------------------------------------------------------------------------------------------------ kernels
+template <typename T, int BT>
+__global__ __launch_bounds__(BT) void k_scan(SampleP P) {
+  __shared__ float smax[BT / 64];
+  __shared__ int sidx[BT / 64];
+  const int r = (int)P.grid_div.div(blockIdx.x), c = (int)blockIdx.x - r * P.grid_chunks;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, base = c * PER * BT;
+  const RowView<T> v = row_view<T>(P.a, r);
+  float x[PER];
+  load_chunk<T, BT>(v, base, tid, x);
+  float top = x[0];
+#pragma unroll
+  for (int e = 1; e < PER; ++e) top = fmaxf(top, x[e]);
+  if (P.want_max) P.tmax[((int64_t)r * P.chunks + c) * BT + tid] = top;
+  int at = 0x7FFFFFFF;
+#pragma unroll
+  for (int e = PER - 1; e >= 0; --e)
+    if (x[e] == top) at = index_at<T, BT>(v.vec, base, tid, e);
+  // (a thread's indexes grow with e, so the last assignment is its lowest)
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const float y = __shfl_xor(top, o);
+    const int j = __shfl_xor(at, o);
+    if (y > top || (y == top && j < at)) {
+      top = y;
+      at = j;
+    }
+  }
+  if (lane == 0) {
+    smax[wave] = top;
+    sidx[wave] = at;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < BT / 64; ++w)
+      if (smax[w] > top || (smax[w] == top && sidx[w] < at)) {
+        top = smax[w];
+        at = sidx[w];
+      }
+    P.cmax[(int64_t)r * P.chunks + c] = top;
+    P.cidx[(int64_t)r * P.chunks + c] = at;
+  }
+  if (c == 0) {  // the row's state and histogram, for the launches behind this one
+    for (int i = tid; i < BINS; i += BT) {
+      P.hist_mass[(int64_t)r * BINS + i] = 0;
+      P.hist_cnt[(int64_t)r * BINS + i] = 0;
+    }
+    if (tid == 0) P.state[r] = RowState{};
+  }
+}
+
+// a row with a small top_k, finished by one block. CT: threads of the blocks whose threads' maxima these are
+template <typename T, int CT>
+__device__ __forceinline__ void finish_small_k(Shared<ST>& S, const SampleP& P, int r, const RowSettings& s, float top) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const RowView<T> v = row_view<T>(P.a, r);
+  const float* const tm = P.tmax + (int64_t)r * P.chunks * CT;
+  const int groups = P.chunks * CT;
+  uint32_t* const pick = reinterpret_cast<uint32_t*>(S.mass);  // groups that may hold one of the k largest
+  constexpr int PICK = 2 * BINS;
+  S.cnt[tid] = 0;
+  S.mass[tid] = 0;
+  if (tid == 0) S.n = S.pick = 0;
+  __syncthreads();
+  for (int g = tid; g < groups; g += ST) {
+    const float x = tm[g];
+    if (x > -INFINITY) atomicAdd(&S.cnt[bin_of(x, top)], 1u);
+  }
+  __syncthreads();
+  find_bin(S, false, (uint32_t)s.top_k, 0.0, 0, 0);
+  const int b = S.sel < 0 ? BINS - 1 : S.sel;  // the k largest values lie in bins up to b
+  for (int g = tid; g < groups; g += ST) {
+    const float x = tm[g];
+    if (x > -INFINITY && bin_of(x, top) <= b) {
+      const int j = atomicAdd(&S.pick, 1);
+      if (j < PICK) pick[j] = (uint32_t)g;
+    }
+  }
+  __syncthreads();
+  const int ng = S.pick;
+  if (ng <= PICK)
+    for (int u = tid; u < ng * PER; u += ST) {
+      const int g = (int)pick[u / PER], c = g / CT;
+      const int i = index_at<T, CT>(v.vec, c * PER * CT, g - c * CT, u % PER);
+      if (i >= v.V) continue;
+      const float x = clean((float)v.p[i]);
+      if (x == -INFINITY || bin_of(x, top) > b) continue;
+      const int j = atomicAdd(&S.n, 1);
+      if (j < CAP) S.list[j] = entry_of(x, i);
+    }
+  __syncthreads();
+  if (ng > PICK || S.n > CAP) {
+    general_row<T, ST>(S, P, r, top);
+    return;
+  }
+  int n = S.n;
+  sort_list(S, n);
+  n = min(n, s.top_k);
+  if (s.has_p) {
+    u64 total = 0, mass;
+    (void)list_reach(S, 0, n, INFINITY, 0, top, P.one, total);
+    n = 1 + list_reach(S, 0, n, (double)s.top_p * (double)total, 0, top, P.one, mass);
+  }
+  // weights at the temperature (the values that min_p drops are the last ones: no weight), then the order of the ids
+  u64 w = 0, e = 0;
+  if (tid < n) {
+    e = S.list[tid];
+    const double rel = rel_of(key_value(entry_key(e)), top);
+    w = rel < s.least ? 0 : weight(rel * s.inv_t, P.one);
+  }
+  __syncthreads();
+  if (tid < n) {
+    S.mass[tid] = w;
+    S.list[tid] = (e << 32) | (uint32_t)tid;
+  }
+  __syncthreads();
+  sort_list(S, n);
+  if (tid >= 64) return;
+  u64 total = 0;
+  for (int i = lane; i < n; i += 64) total += S.mass[i];
+  total = wave_sum64(total);
+  const double target = draw_target(P.a.u[r], total);
+  const bool past = !((double)total > target);
+  u64 before = 0, wt = 0;
+  int tok = -1;
+  for (int i = 0; i < n; i += 64) {
+    const u64 q = i + lane < n ? S.list[i + lane] : 0;
+    const u64 m = i + lane < n ? S.mass[(uint32_t)q] : 0, mi = before + wave_scan64(m, lane);
+    const uint64_t who = __ballot(past ? m != 0 : (double)mi > target);
+    before = __shfl(mi, 63);
+    if (!who) continue;
+    const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
+    tok = (int)(__shfl(q, l) >> 32);
+    wt = __shfl(m, l);
+    if (!past) break;
+  }
+  if (lane == 0) put(P, r, tok, wt, total);
+}
+
+static_assert(ST == BINS, "one bin a thread");
+template <typename T, int CT>
+__global__ __launch_bounds__(ST) void k_select(SampleP P) {
+  __shared__ Shared<ST> S;
+  const int r = (int)P.grid_div.div(blockIdx.x), c = (int)blockIdx.x - r * P.grid_chunks;
+  const RowSettings s = settings_of(P.a, r);
+  if (s.kind != HIST && !(s.kind == SMALL_K && c == 0)) return;
+  int at;
+  const float top = row_top(S, P, r, at);
+  if (top == -INFINITY) {  // (HIST: k_draw answers)
+    if (s.kind == SMALL_K && threadIdx.x == 0) {
+      P.a.token_out[r] = -1;
+      if (P.a.prob_out) P.a.prob_out[r] = 0.f;
+    }
+    return;
+  }
+  if (s.kind == SMALL_K) {
+    finish_small_k<T, CT>(S, P, r, s, top);
+    return;
+  }
+  const int tid = threadIdx.x;
+  S.cnt[tid] = 0;
+  S.mass[tid] = 0;
+  float x[PER];
+  load_chunk<T, ST>(row_view<T>(P.a, r), c * PER * ST, tid, x);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    if (x[e] == -INFINITY) continue;
+    const int b = bin_of(x[e], top);
+    atomicAdd(&S.cnt[b], 1u);
+    if (s.has_p) atomicAdd(&S.mass[b], weight(rel_of(x[e], top), P.one));
+  }
+  __syncthreads();
+  u64* const hm = P.hist_mass + (int64_t)r * BINS;
+  uint32_t* const hc = P.hist_cnt + (int64_t)r * BINS;
+  if (S.cnt[tid]) dev_add(hc + tid, S.cnt[tid]);
+  if (S.mass[tid]) dev_add(hm + tid, S.mass[tid]);
+  RowState* const st = P.state + r;
+  if (!last_to_arrive(S, &st->arrived_select, P.sel_chunks)) return;
+  S.cnt[tid] = dev_load(hc + tid);
+  S.mass[tid] = dev_load(hm + tid);
+  __syncthreads();
+  // the bins of the cuts. top_k's lies in b_k. top_p's target is p of the top_k's mass, which is known but for b_k's share:
+  // it lies in the bins between the targets at both ends
+  int b_lo = -1, b_hi = -1, b_k = -1;
+  u64 mass_lo = 0, mass_k = 0;
+  uint32_t cnt_k = 0;
+  if (s.has_k) {
+    find_bin(S, false, (uint32_t)s.top_k, 0.0, 0, 0);
+    b_k = S.sel;
+    if (b_k >= 0) {
+      cnt_k = S.before_cnt;
+      mass_k = S.before_mass;
+    }
+  } else {
+    find_bin(S, true, 0, INFINITY, 0, 0);
+  }
+  u64 total = S.total;
+  const u64 in_k = b_k >= 0 ? S.mass[b_k] : 0;
+  __syncthreads();
+  if (s.has_p) {
+    const double lo = (double)s.top_p * (double)(b_k >= 0 ? mass_k : total);
+    const double hi = (double)s.top_p * (double)(b_k >= 0 ? mass_k + in_k : total);
+    find_bin(S, true, 0, lo, 0, 0);
+    b_lo = S.sel;
+    mass_lo = S.before_mass;
+    __syncthreads();
+    find_bin(S, true, 0, hi, 0, 0);
+    b_hi = S.sel;
+  } else {
+    b_lo = b_hi = b_k;  // (none: fewer than k values, everything is kept)
+    mass_lo = mass_k;
+  }
+  if (tid == 0) {
+    uint32_t n = 0;
+    if (b_lo >= 0)
+      for (int i = b_lo; i <= b_hi; ++i) n += S.cnt[i];
+    if (b_k > b_hi) n += S.cnt[b_k];
+    st->overflow = n > CAP;
+    st->b_lo = b_lo < 0 ? BINS : b_lo;  // bins below b_lo are kept whole
+    st->b_hi = b_hi;
+    st->b_k = b_k;
+    st->mass_lo = mass_lo;
+    st->mass_k = mass_k;
+    st->cnt_k = cnt_k;
+    st->total = total;
+  }
+}
+
+template <typename T, int BT>
+__global__ __launch_bounds__(BT, BT == 256 ? 4 : 1) void k_draw(SampleP P) {
+  __shared__ Shared<BT> S;
+  const int r = (int)P.grid_div.div(blockIdx.x), c = (int)blockIdx.x - r * P.grid_chunks;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const RowSettings s = settings_of(P.a, r);
+  if (s.kind == SMALL_K || (s.kind == GREEDY && c != 0)) return;
+  int at;
+  const float top = row_top(S, P, r, at);
+  if (s.kind == GREEDY || top == -INFINITY) {
+    if (c == 0 && tid == 0) {
+      P.a.token_out[r] = top == -INFINITY ? -1 : at;
+      if (P.a.prob_out) P.a.prob_out[r] = top == -INFINITY ? 0.f : 1.f;
+    }
+    return;
+  }
+  RowState* const st = P.state + r;
+  const bool hist = s.kind == HIST;
+  if (hist && st->overflow) {
+    if (c == 0) general_row<T, BT>(S, P, r, top);
+    return;
+  }
+  const int b_lo = hist ? st->b_lo : BINS, b_hi = hist ? st->b_hi : -1, b_k = hist ? st->b_k : -1;
+  const RowView<T> v = row_view<T>(P.a, r);
+  float x[PER];
+  load_chunk<T, BT>(v, c * PER * BT, tid, x);
+  u64 sum = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const bool some = x[e] > -INFINITY;
+    const int b = some ? bin_of(x[e], top) : BINS;
+    if (b < b_lo && some) {
+      const double rel = rel_of(x[e], top);
+      if (!(rel < s.least)) sum += weight(rel * s.inv_t, P.one);
+    }
+    const bool listed = some && ((b >= b_lo && b <= b_hi) || b == b_k);
+    const uint64_t who = __ballot(listed);
+    if (who) {
+      uint32_t j = 0;
+      if (lane == first_lane(who)) j = dev_add(&st->list_n, (uint32_t)__popcll(who));
+      j = __shfl(j, first_lane(who)) + __popcll(who & ((1ull << lane) - 1));
+      if (listed && j < CAP) dev_store(P.list + (int64_t)r * CAP + j, entry_of(x[e], index_at<T, BT>(v.vec, c * PER * BT, tid, e)));
+    }
+  }
+  sum = wave_sum64(sum);
+  if (lane == 0) S.part[wave] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < BT / 64; ++w) sum += S.part[w];
+    dev_store(P.cmass + (int64_t)r * P.chunks + c, sum);
+  }
+  if (!last_to_arrive(S, &st->arrived_draw, P.chunks)) return;
+
+  // the cut
+  Cut cut{0, 0x7FFFFFFF};
+  const int n = hist ? (int)dev_load(&st->list_n) : 0;
+  u64* const cm = P.cmass + (int64_t)r * P.chunks;
+  if (n > 0) {
+    for (int i = tid; i < n; i += BT) S.list[i] = dev_load(P.list + (int64_t)r * CAP + i);
+    __syncthreads();
+    sort_list(S, n);
+    int end = n;  // listed values within top_k
+    u64 total = st->total;
+    if (b_k >= 0) {
+      // the first listed value in bin b_k: everything in front of it lies in lower bins
+      int lo = 0, hi = n;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (bin_of(key_value(entry_key(S.list[mid])), top) < b_k) lo = mid + 1;
+        else hi = mid;
+      }
+      end = lo + (s.top_k - (int)st->cnt_k);
+      if (s.has_p) (void)list_reach(S, lo, end, INFINITY, st->mass_k, top, P.one, total);
+    }
+    int last = end - 1;
+    if (s.has_p) {
+      u64 mass;
+      last = list_reach(S, 0, end, (double)s.top_p * (double)total, st->mass_lo, top, P.one, mass);
+    }
+    cut = Cut{entry_key(S.list[last]), (int)(uint32_t)S.list[last]};
+    // the kept ones' mass goes to their chunks (this block alone is left; its accesses go the same way as the others')
+    for (int i = tid; i <= last; i += BT) {
+      const double rel = rel_of(key_value(entry_key(S.list[i])), top);
+      if (!(rel < s.least))
+        dev_add(cm + (uint32_t)S.list[i] / (PER * BT), weight(rel * s.inv_t, P.one));
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+  // the chunk
+  if (wave == 0) {
+    u64 total = 0;
+    for (int i = lane; i < P.chunks; i += 64) total += dev_load(cm + i);
+    total = wave_sum64(total);
+    const double target = draw_target(P.a.u[r], total);
+    const bool past = !((double)total > target);
+    u64 before = 0, found = 0;
+    int pick = -1;
+    for (int i = 0; i < P.chunks; i += 64) {
+      const u64 w = i + lane < P.chunks ? dev_load(cm + i + lane) : 0;
+      const u64 mi = before + wave_scan64(w, lane);
+      const uint64_t who = __ballot(past ? w != 0 : (double)mi > target);
+      if (who) {
+        const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
+        pick = i + l;
+        found = __shfl(mi - w, l);
+        if (!past) break;
+      }
+      before = __shfl(mi, 63);
+    }
+    if (lane == 0) {
+      S.pick = pick;
+      S.chunk_before = found;
+      S.total = total;
+    }
+  }
+  __syncthreads();
+  // the token: sums of 64 W consecutive values in the order of the vocabulary, then the lane, then the value
+  const int pick = S.pick, base = pick * PER * BT;
+  const u64 total = S.total;
+  const double target = draw_target(P.a.u[r], total);
+  const bool past = !((double)total > target);
+  load_chunk<T, BT>(v, base, tid, x);
+  u64 w[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    w[e] = 0;
+    const int i = index_at<T, BT>(v.vec, base, tid, e);
+    if (x[e] > -INFINITY && within(order_key(x[e]), i, cut)) {
+      const double rel = rel_of(x[e], top);
+      if (!(rel < s.least)) w[e] = weight(rel * s.inv_t, P.one);
+    }
+  }
+  constexpr int NW = BT / 64;
+  const int W = v.vec ? kWide<T> : 1, runs = PER / W;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {  // a lane's sum of each run in w's last place of the run
+    if (e % W) w[e] += w[e - 1];
+    if (e % W == W - 1) {
+      const u64 t = wave_sum64(w[e]);
+      if (lane == 0) S.part[(e / W) * NW + wave] = t;
+    }
+  }
+  __syncthreads();
+  u64 before = S.chunk_before;
+  int cell = -1;
+  for (int i = 0; i < runs * NW; ++i) {
+    const u64 t = S.part[i];
+    if (past ? t != 0 : (double)(before + t) > target) {
+      cell = i;
+      if (!past) break;
+    }
+    if (!past) before += t;
+  }
+  if (cell < 0 || wave != cell % NW) return;
+  const int run = cell / NW;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    if (e / W != run || e % W != W - 1) continue;
+    const u64 mi = before + wave_scan64(w[e], lane);
+    const uint64_t who = __ballot(past ? w[e] != 0 : (double)mi > target);
+    const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
+    if (lane != l) continue;
+    // the value within the lane's run (w holds running sums)
+    const u64 b0 = mi - w[e];
+    int hit = -1;
+    u64 wt = 0;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      if (q / W != run) continue;
+      const u64 prev = q % W ? w[q - 1] : 0, own = w[q] - prev;
+      if (own && (past || (hit < 0 && (double)(b0 + w[q]) > target))) {
+        hit = q;
+        wt = own;
+      }
+    }
+    put(P, r, index_at<T, BT>(v.vec, base, tid, hit), wt, total);
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------------------- host
+struct SamplePlan {
   SampleP P;
-  P.a = *ap;
-  const fa_sample_args& a = P.a;
+  int bt;
+  bool select, draw;
+  int select_blocks, draw_blocks;  // a row
+  int64_t bytes;
+};
+
+static SamplePlan sample_plan(const fa_sample_args* ap) {
+  FA_REQUIRE(ap, "sample_tokens: no arguments");
+  SamplePlan t;
+  t.P.a = *ap;
+  const fa_sample_args& a = t.P.a;
   FA_REQUIRE(a.rows >= 0 && a.vocab >= 1 && a.vocab <= (1 << 24), "sample_tokens: rows, or vocab outside 1 .. 2^24");
   FA_REQUIRE(a.type == FA_F32 || a.type == FA_F16 || a.type == FA_BF16, "sample_tokens: type");
   FA_REQUIRE(a.row_stride >= a.vocab || a.rows <= 1, "sample_tokens: rows overlap");
   int lg = 0;
   while ((1 << lg) < a.vocab) ++lg;
-  P.one = (double)(1ull << (62 - lg));
-  return P;
+  t.P.one = (double)(1ull << (62 - lg));
+  // 256 threads a block where that still leaves the launch at up to four blocks a compute unit, else 1024
+  const int64_t small = (a.vocab + PER * 256 - 1) / (PER * 256);
+  t.bt = a.rows * small <= 1024 ? 256 : 1024;
+  t.P.chunks = (a.vocab + PER * t.bt - 1) / (PER * t.bt);
+  t.P.sel_chunks = (a.vocab + PER * ST - 1) / (PER * ST);
+  FA_REQUIRE((int64_t)a.rows * t.P.chunks < (1ll << 31), "sample_tokens: more than 2^31 chunks");
+  // which launches the rows can need (settings of each row live on the device: all)
+  const bool each = a.temperatures || a.top_ps || a.min_ps || a.top_ks;
+  const bool greedy = !(a.temperature > 0.f) || a.top_k == 1 || !(a.top_p > 0.f) || !(a.min_p <= 1.f);
+  const bool has_k = a.top_k > 0 && a.top_k < a.vocab, small_k = has_k && a.top_k <= KMAX;
+  t.select = each || (!greedy && (has_k || a.top_p < 1.f));
+  t.draw = each || greedy || !small_k;
+  t.P.want_max = each || (!greedy && small_k);
+  t.select_blocks = each || !small_k ? t.P.sel_chunks : 1;
+  t.draw_blocks = each || !greedy ? t.P.chunks : 1;
+  const int64_t n = a.rows, nc = n * t.P.chunks;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t x = at;
+    at += (bytes + 255) / 256 * 256;
+    return x;
+  };
+  char* const ws = reinterpret_cast<char*>(a.workspace);
+  t.P.state = reinterpret_cast<RowState*>(ws + take(n * sizeof(RowState)));
+  t.P.hist_mass = reinterpret_cast<u64*>(ws + take(n * BINS * 8));
+  t.P.hist_cnt = reinterpret_cast<uint32_t*>(ws + take(n * BINS * 4));
+  t.P.list = reinterpret_cast<u64*>(ws + take(n * CAP * 8));
+  t.P.cmass = reinterpret_cast<u64*>(ws + take(nc * 8));
+  t.P.cmax = reinterpret_cast<float*>(ws + take(nc * 4));
+  t.P.cidx = reinterpret_cast<int*>(ws + take(nc * 4));
+  t.P.tmax = reinterpret_cast<float*>(ws + take(t.P.want_max ? nc * t.bt * 4 : 0));
+  t.bytes = at;
+  return t;
+}
+
+template <typename T, int BT>
+static void sample_run(const SamplePlan& t, hipStream_t s) {
+  auto go = [&](void (*kernel)(SampleP), int blocks, int threads) {
+    SampleP P = t.P;
+    P.grid_chunks = blocks;
+    P.grid_div = FastDiv::of((uint32_t)blocks);
+    launch(kernel, dim3((uint32_t)P.a.rows * (uint32_t)blocks), dim3(threads), 0, s, P);
+  };
+  go(k_scan<T, BT>, t.P.chunks, BT);
+  if (t.select) go(k_select<T, BT>, t.select_blocks, ST);
+  if (t.draw) go(k_draw<T, BT>, t.draw_blocks, BT);
 }
 
 static void sample_tokens(const fa_sample_args* ap, hipStream_t s) {
-  SampleP P = sample_plan(ap);
-  const fa_sample_args& a = P.a;
+  const SamplePlan t = sample_plan(ap);
+  const fa_sample_args& a = t.P.a;
   if (a.rows == 0) return;
   FA_REQUIRE(a.logits && a.u && a.token_out, "sample_tokens: null tensor");
-  auto k = a.type == FA_F32 ? k_sample_row<float> : a.type == FA_F16 ? k_sample_row<_Float16> : k_sample_row<__bf16>;
-  launch(k, dim3(a.rows), dim3(ST), 0, s, P);
+  FA_REQUIRE(a.workspace && a.workspace_bytes >= t.bytes && aligned16(a.workspace),
+             "sample_tokens: workspace too small or not 16-byte aligned");
+  if (a.type == FA_F32) t.bt == 256 ? sample_run<float, 256>(t, s) : sample_run<float, 1024>(t, s);
+  else if (a.type == FA_F16) t.bt == 256 ? sample_run<_Float16, 256>(t, s) : sample_run<_Float16, 1024>(t, s);
+  else t.bt == 256 ? sample_run<__bf16, 256>(t, s) : sample_run<__bf16, 1024>(t, s);
 }
 
 }  // namespace fa
@@ -456,8 +1076,7 @@ extern "C" {
 int fa_sample_tokens_workspace(const fa_sample_args* a, int64_t* bytes) {
   FA_API_BEGIN
   FA_REQUIRE(bytes, "sample_tokens: no place for the size");
-  (void)fa::sample_plan(a);
-  *bytes = 0;
+  *bytes = fa::sample_plan(a).bytes;
   FA_API_END
 }
 
