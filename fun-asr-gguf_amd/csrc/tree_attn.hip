@@ -2,17 +2,23 @@
 //
 // For one sequence and kv head the rows are (drafted token, query head of the group), all of which read the same keys:
 //   S = K Q^T,  P = softmax over keys (running maximum and sum, 32 bits),  O^T += V^T P^T.
-// A block takes up to 16 RT of those rows and one chunk of the keys; its four waves take every fourth 32-key tile of the
-// chunk, each with a running maximum, sum and output of its own, and join at the end through LDS. Blocks of the same rows
-// leave partial results (unnormalised output, maximum, sum) that k_tree_merge joins.
-//
-// Both products run on 16x16x32 matrix instructions. S is made with the keys as rows, so that a lane's results belong to
-// one query row (lane % 16) and 4 consecutive keys, in two tiles 8: exactly the operand P^T of the second product, whose
+// Both products run on 16x16x32 matrix instructions. S is made with the keys as rows, so that a lane's results belong to one
+// query row (lane % 16) and 4 consecutive keys, in two tiles 8: exactly the operand P^T of the second product, whose
 // contraction runs over the keys in that order (4 g + i, then 16 + 4 g + i); V^T is read from LDS in the same order by the
 // transposing reads. The output's columns are query rows too, so rescaling needs no exchange between lanes; the running
-// maximum needs two. K goes from memory straight into operand registers (a key row is read in 64-byte pieces by 4 lanes),
-// V through wave-private LDS whose 32-byte pairs are permuted by the key (pair ^ key % 8): the 16 rows that a transposing
-// read touches then cover all banks evenly.
+// maximum needs two.
+//
+// Two kernels, by the number of rows of a sequence and kv head:
+//   k_few (up to 32): what bounds it is reading K and V once. The four waves of a block take every fourth 32-key tile of the
+//     block's keys, each with a running maximum, sum and output of its own, and join through LDS at the end: no barrier in
+//     the loop. K goes from memory straight into operand registers (a key row in 64-byte pieces by 4 lanes), V through
+//     wave-private LDS.
+//   k_many: the softmax's vector instructions weigh as much as the reading. The block's waves take 16 RT rows each and share
+//     every K and V tile through two LDS stages, so a tile is read once for 64 RT rows; one barrier a tile.
+// In LDS, row k's 16-byte piece j lies at j ^ (k mod pieces): an operand read's 16 rows, and a transposing read's 16 rows of
+// 32 bytes, then cover all banks evenly.
+// Blocks of the same rows split the keys where the launch would not fill the card; k_tree_merge joins their partial results
+// (unnormalised output, maximum, sum).
 #include "api.h"
 #include "draft_ops.h"
 
@@ -26,14 +32,15 @@ typedef short v4i16 __attribute__((ext_vector_type(4)));
 
 struct TreeP {
   fa_tree_attention_args a;
-  FastDiv page_div, group_div;
+  FastDiv page_div, group_div, q_tiles_div, kv_div, splits_div;
   int group, rows;     // query heads per kv head; rows of one sequence and kv head: nodes * group
-  int q_tiles;         // blocks of 16 RT rows
-  int chunk, splits;   // keys per block (a multiple of 128), blocks along the keys at most
+  int q_tiles;         // blocks along the rows
+  int chunk, splits;   // keys a block (a multiple of 128), blocks along the keys at most
+  int n_groups;        // (sequence, kv head, split) triples
   float c;             // scale * log2(e)
   float* part_o;       // [seqs][kv_heads][splits][rows][DP]
   float* part_ml;      // [seqs][kv_heads][splits][rows][2]
-  int q_vec, out_vec;  // q / out rows may be accessed in 16-byte pieces
+  int q_vec;           // q's rows may be read in 16-byte pieces
 };
 
 __device__ __forceinline__ f32x4 mfma16(f16x8_t a, f16x8_t b, f32x4 c) {
@@ -42,10 +49,9 @@ __device__ __forceinline__ f32x4 mfma16(f16x8_t a, f16x8_t b, f32x4 c) {
 __device__ __forceinline__ f32x4 mfma16(bf16x8_t a, bf16x8_t b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ v4i16 ld_tr(const void* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(p));
-}
-// maximum / sum over the four 16-lane groups of a wave
+// 2^x; results below 2^-126 become 0 (weights that far under the row's largest)
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// over the four 16-lane groups of a wave
 __device__ __forceinline__ float across_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
   return fmaxf(v, __shfl_xor(v, 32));
@@ -54,8 +60,7 @@ __device__ __forceinline__ float across_sum(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
 }
-// exponent bits of a 16-bit type, both halves of a register
-template <typename T> constexpr uint32_t kExp = 0;
+template <typename T> constexpr uint32_t kExp = 0;  // exponent bits
 template <> constexpr uint32_t kExp<_Float16> = 0x7C00u;
 template <> constexpr uint32_t kExp<__bf16> = 0x7F80u;
 
@@ -73,71 +78,229 @@ __device__ __forceinline__ SeqLens seq_lens(const TreeP& P, int b) {
   return s;
 }
 
-// T: cache type. NS: 16-bit terms of q and of the probabilities (1: q is of the cache's type; 2 / 3: q is float32, kept to
-// 22 / 24 bits by terms of float16 / bfloat16). DP: head_dim rounded up to 64 / 128 / 256.
-template <typename T, int NS, int DP, int RT>
-__global__ __launch_bounds__(256) void k_tree_attn(TreeP P) {
+// The block's part: consecutive block numbers go round the XCDs, so the row tiles of one (sequence, kv head, split), which
+// read the same keys, are 8 numbers apart: one XCD's L2 fetches those keys once. false: a block of the round-up
+struct Where {
+  int b, h, split, q_tile;
+};
+__device__ __forceinline__ bool locate(const TreeP& P, Where& w) {
+  const uint32_t xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, g8 = P.q_tiles_div.div(slot);
+  w.q_tile = (int)(slot - g8 * P.q_tiles);
+  const uint32_t g = g8 * 8 + xcd;
+  if (g >= (uint32_t)P.n_groups) return false;
+  const uint32_t bh = P.splits_div.div(g);
+  w.split = (int)(g - bh * P.splits);
+  w.b = (int)P.kv_div.div(bh);
+  w.h = (int)(bh - (uint32_t)w.b * P.a.kv_heads);
+  return true;
+}
+
+// this lane's query row (of rows r0 + r16) as NS terms of the cache's type: dimensions 8 (g4 + 4 ks) + 0 .. 7
+template <typename T, int NS, int KS>
+__device__ __forceinline__ int load_q(const TreeP& P, const Where& w, int rr, int rows, int g4,
+                                      typename Vec8<T>::type (&q)[KS][NS]) {
+  const fa_tree_attention_args& a = P.a;
+  const int rc = min(rr, rows - 1), node = (int)P.group_div.div((uint32_t)rc);
+  const int64_t at = w.b * a.q_seq + node * a.q_node + (int64_t)(w.h * P.group + rc - node * P.group) * a.q_head;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int e = 8 * (g4 + 4 * ks);
+    float x[8] = {};
+    if (rr < rows && e < a.head_dim) {
+      if constexpr (NS > 1) {
+        const float* p = reinterpret_cast<const float*>(a.q) + at + e;
+        if (P.q_vec) load8<true>(p, x);
+        else load8<false>(p, x);
+      } else {
+        const T* p = reinterpret_cast<const T*>(a.q) + at + e;
+        if (P.q_vec) load8<true>(p, x);
+        else load8<false>(p, x);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const T y = (T)x[i];
+        q[ks][s][i] = y;
+        x[i] -= (float)y;
+      }
+  }
+  return node;
+}
+
+// which of this lane's 8 keys of a 32-key group the row sees: bit i: key 16 (i / 4) + 4 g4 + i % 4 of the group at kt.
+// present: the group's keys that exist
+__device__ __forceinline__ uint32_t seen_bits(const TreeP& P, int b, int ctx, int kt, uint32_t present, int node, int g4) {
+  const fa_tree_attention_args& a = P.a;
+  uint32_t bits = 0;
+  const uint8_t* const row = a.mask ? a.mask + b * a.mask_seq + node * a.mask_row : nullptr;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int kk = 16 * (i >> 2) + 4 * g4 + (i & 3), j = kt + kk - ctx;
+    const uint32_t drafted = row ? row[min(max(j, 0), a.nodes - 1)] != 0 : j <= node;
+    bits |= ((present >> kk) & (j < 0 ? 1u : drafted) & 1u) << i;
+  }
+  return bits;
+}
+
+// One group of 32 keys of the softmax: scores s -> weights e relative to the running maximum; o and l rescaled
+template <int MT>
+__device__ __forceinline__ void softmax_step(const f32x4 (&s)[2], float c, float& m, float& l, f32x4 (&o)[MT], float (&e)[8]) {
+  float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                    fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+  top = fmaxf(m, across_max(top));
+  const float base = (top == -INFINITY ? 0.f : top) * c;  // nothing seen so far: every weight is 2^-inf = 0
+  const float alpha = exp2_fast(m * c - base);
+  if (__any(top != m)) {  // (first tiles mostly)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) o[mt] *= alpha;
+    l *= alpha;
+  }
+  m = top;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    e[i] = exp2_fast(fmaf(s[i >> 2][i & 3], c, -base));
+    sum += e[i];
+  }
+  l += sum;
+}
+template <typename T, int NS>
+__device__ __forceinline__ void to_terms(float (&e)[8], typename Vec8<T>::type (&p)[NS]) {
+#pragma unroll
+  for (int n = 0; n < NS; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T y = (T)e[i];
+      p[n][i] = y;
+      e[i] -= (float)y;
+    }
+}
+
+// sets the infinities and NaN among 8 values to 0; true if there were any
+template <typename T>
+__device__ __forceinline__ bool strip_nonfinite(typename Vec8<T>::type& v) {
+  uint4 u = __builtin_bit_cast(uint4, v);
+  constexpr uint32_t E = kExp<T>;
+  uint32_t hit = 0;
+  for (uint32_t* x : {&u.x, &u.y, &u.z, &u.w}) {
+    const uint32_t lo = (*x & E) == E ? 0xFFFFu : 0u, hi = (*x >> 16 & E) == E ? 0xFFFF0000u : 0u;
+    hit |= lo | hi;
+    *x &= ~(lo | hi);
+  }
+  v = __builtin_bit_cast(typename Vec8<T>::type, u);
+  return hit != 0;
+}
+
+__device__ __forceinline__ void apply_mask(uint32_t bits, f32x4 (&s)[2]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] = (bits >> i) & 1 ? s[i >> 2][i & 3] : -INFINITY;
+}
+
+// An infinity or NaN in a drafted key's value must reach the rows that have a weight for it and no others (in the matrix
+// product 0 * inf would reach every row): the loops leave such values out (strip_nonfinite), and where there were any, this
+// adds them at the end, key by key, for the 32-key groups kt, kt + step ... of the drafted keys. wl: 32 x 16 floats of LDS of
+// the wave's own. Rare, and kept out of the loops for their registers' sake.
+template <typename T, int NS, int DP>
+__device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, const SeqLens& L, int kt, int k1, int step,
+                                              int node, const typename Vec8<T>::type (&q)[DP / 32][NS], float m, float* wl,
+                                              f32x4 (&o)[DP / 16]) {
   typedef typename Vec8<T>::type V8;
-  constexpr int KS = DP / 32, MT = DP / 16, ROWS = 16 * RT;
+  const fa_tree_attention_args& a = P.a;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
+  const T* const kbase = reinterpret_cast<const T*>(a.k_cache) + w.h * a.k_head;
+  const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + w.h * a.v_head;
+  const int32_t* const table = a.block_table + w.b * a.table_seq;
+  const float base = (m == -INFINITY ? 0.f : m) * P.c;
+  for (; kt < k1; kt += step) {
+    if (kt + 32 <= L.ctx) continue;
+    f32x4 s[2];
+    uint32_t present = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int key = kt + 16 * t + r16;
+      const uint32_t pg = P.page_div.div((uint32_t)key);
+      const int id = key < k1 ? table[pg] : -1;
+      const bool ok = (uint32_t)id < (uint32_t)a.pages;
+      present |= (uint32_t)(__ballot(ok) & 0xFFFF) << (16 * t);
+      const T* const k = ok ? kbase + id * a.k_page + (int64_t)((uint32_t)key - pg * a.page_size) * a.k_slot : kbase;
+      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < DP / 32; ++ks) {
+        const int e = 8 * (g4 + 4 * ks);
+        const V8 x = *reinterpret_cast<const V8*>(k + (e < a.head_dim ? e : 0));
+#pragma unroll
+        for (int n = NS - 1; n >= 0; --n) s[t] = mfma16(x, q[ks][n], s[t]);
+      }
+    }
+    apply_mask(seen_bits(P, w.b, L.ctx, kt, present, node, g4), s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      wl[(16 * (i >> 2) + 4 * g4 + (i & 3)) * 16 + r16] = exp2_fast(fmaf(s[i >> 2][i & 3], P.c, -base));
+    for (int k = 0; k < 32 && kt + k < k1; ++k) {
+      if (kt + k < L.ctx) continue;
+      const uint32_t pg = P.page_div.div((uint32_t)(kt + k));
+      const int id = table[pg];
+      if ((uint32_t)id >= (uint32_t)a.pages) continue;
+      const T* const v = vbase + id * a.v_page + (int64_t)((uint32_t)(kt + k) - pg * a.page_size) * a.v_slot;
+      const float f = wl[k * 16 + r16];
+#pragma unroll
+      for (int mt = 0; mt < DP / 16; ++mt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int d = 16 * mt + 4 * g4 + j;
+          const float x = d < a.head_dim ? (float)v[d] : 0.f;
+          if (!(fabsf(x) < INFINITY) && f != 0.f) o[mt][j] += f * x;
+        }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ typename Vec8<T>::type values_operand(const T* lo, const T* hi) {
+  typename Vec8<T>::type v;
+  const v4i16 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(lo));
+  const v4i16 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(hi));
+  const auto p = __builtin_bit_cast(T __attribute__((ext_vector_type(4))), x);
+  const auto q = __builtin_bit_cast(T __attribute__((ext_vector_type(4))), y);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = p[i];
+    v[4 + i] = q[i];
+  }
+  return v;
+}
+
+template <typename TO>
+__device__ __forceinline__ void store4(TO* p, f32x4 x, int left) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < left) p[i] = (TO)x[i];
+}
+
+// T: cache type. NS: 16-bit terms of q and of the probabilities (1: q is of the cache's type; 2 / 3: q is float32, kept to 22 /
+// 24 bits by terms of float16 / bfloat16; with 1 term the weights are rounded to the cache's type, half a step of it, as the
+// output is). DP: head_dim rounded up to 64 / 128 / 256. FULL: it is DP itself; else a piece behind head_dim is read at 0
+// instead (q is 0 there, and the output's dimensions behind it are not written).
+template <typename T, int NS, int DP, int RT, bool FULL>
+__global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_few(TreeP P) {
+  typedef typename Vec8<T>::type V8;
+  constexpr int KS = DP / 32, MT = DP / 16, ROWS = 16 * RT, PIECES = DP / 8;
   constexpr int OS = DP + 4;  // output rows in LDS: 16 rows of a float4 store on different banks
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const fa_tree_attention_args& a = P.a;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g4 = lane >> 4;
-  const int b = blockIdx.z, h = blockIdx.y % a.kv_heads, qt = blockIdx.y / a.kv_heads, split = blockIdx.x;
-  const SeqLens L = seq_lens(P, b);
-  const int rows = L.n * P.group, r0 = qt * ROWS;
-  if (r0 >= rows || split >= L.splits) return;
+  Where w;
+  if (!locate(P, w)) return;
+  const SeqLens L = seq_lens(P, w.b);
+  const int rows = L.n * P.group, r0 = w.q_tile * ROWS;
+  if (r0 >= rows || w.split >= L.splits) return;
   const int D = a.head_dim;
-  const int k0 = split * P.chunk, k1 = split == L.splits - 1 ? L.total : min(L.total, k0 + P.chunk);
-
-  // this lane's query rows, their operands
-  int node[RT];
-  V8 q[RT][KS][NS];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int rr = r0 + 16 * rt + r16;
-    const int rc = min(rr, rows - 1);
-    node[rt] = (int)P.group_div.div((uint32_t)rc);
-    const int64_t at = b * a.q_seq + node[rt] * a.q_node + (int64_t)(h * P.group + rc - node[rt] * P.group) * a.q_head;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int e = 8 * (g4 + 4 * ks);
-      float x[8] = {};
-      if (rr < rows && e < D) {
-        if constexpr (NS > 1) {
-          const float* p = reinterpret_cast<const float*>(a.q) + at + e;
-          if (P.q_vec) load8<true>(p, x);
-          else load8<false>(p, x);
-        } else {
-          const T* p = reinterpret_cast<const T*>(a.q) + at + e;
-          if (P.q_vec) load8<true>(p, x);
-          else load8<false>(p, x);
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const T y = (T)x[i];
-          q[rt][ks][s][i] = y;
-          x[i] -= (float)y;
-        }
-    }
-  }
-
-  float m[RT], l[RT];
-  f32x4 o[RT][MT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY;
-    l[rt] = 0.f;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) o[rt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  const T* const kbase = reinterpret_cast<const T*>(a.k_cache) + h * a.k_head;
-  const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + h * a.v_head;
-  const int32_t* const table = a.block_table + b * a.table_seq;
+  const int k0 = w.split * P.chunk, k1 = w.split == L.splits - 1 ? L.total : min(L.total, k0 + P.chunk);
+  const T* const kbase = reinterpret_cast<const T*>(a.k_cache) + w.h * a.k_head;
+  const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + w.h * a.v_head;
+  const int32_t* const table = a.block_table + w.b * a.table_seq;
   T* const vl = reinterpret_cast<T*>(smem) + wave * 32 * DP;
 
   // page numbers of this lane's two keys of a tile (16 t + r16): -1 behind the end
@@ -149,26 +312,26 @@ __global__ __launch_bounds__(256) void k_tree_attn(TreeP P) {
     }
   };
   V8 kr[2][KS], vr[2][KS];
-  bool ok[2];
+  uint32_t present = 0;
   // every lane loads: one without a key of its own reads page 0, slot 0 (there is one), which the masks then leave out
   auto issue = [&](int kt, const int (&pid)[2]) {
+    bool ok[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const uint32_t key = (uint32_t)(kt + 16 * t + r16);
-      ok[t] = pid[t] >= 0 && pid[t] < a.pages;
-      const int64_t page = ok[t] ? pid[t] : 0;
-      const int64_t off = ok[t] ? key - P.page_div.div(key) * a.page_size : 0;
-      const T* kp = kbase + page * a.k_page + off * a.k_slot;
-      const T* vp = vbase + page * a.v_page + off * a.v_slot;
+      ok[t] = (uint32_t)pid[t] < (uint32_t)a.pages;
+      const int page = ok[t] ? pid[t] : 0, off = ok[t] ? (int)(key - P.page_div.div(key) * a.page_size) : 0;
+      const T* const kp = kbase + page * a.k_page + off * a.k_slot;
+      const T* const vp = vbase + page * a.v_page + off * a.v_slot;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int e = 8 * (g4 + 4 * ks);
-        kr[t][ks] = *reinterpret_cast<const V8*>(kp + (e < D ? e : 0));
-        vr[t][ks] = *reinterpret_cast<const V8*>(vp + (e < D ? e : 0));
+        const int e = 8 * (g4 + 4 * ks), ec = FULL || e < D ? e : 0;
+        kr[t][ks] = *reinterpret_cast<const V8*>(kp + ec);
+        vr[t][ks] = *reinterpret_cast<const V8*>(vp + ec);
       }
     }
+    present = (uint32_t)(__ballot(ok[0]) & 0xFFFF) | (uint32_t)(__ballot(ok[1]) << 16);
   };
-
   int pid[2];
   int kt = k0 + 32 * wave;
   if (kt < k1) {
@@ -176,18 +339,24 @@ __global__ __launch_bounds__(256) void k_tree_attn(TreeP P) {
     issue(kt, pid);
     page_ids(kt + 128, pid);
   }
+
+  int node[RT];
+  V8 q[RT][KS][NS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) node[rt] = load_q<T, NS, KS>(P, w, r0 + 16 * rt + r16, rows, g4, q[rt]);
+  float m[RT], l[RT];
+  f32x4 o[RT][MT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) o[rt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  bool bad = false;
   for (; kt < k1; kt += 128) {
-    if (D != DP) {  // dimensions behind the head's: zero
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        if (8 * (g4 + 4 * ks) >= D)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) kr[t][ks][i] = vr[t][ks][i] = (T)0.f;
-    }
-    // S: 32 keys x rows
-    f32x4 s[RT][2];
+    f32x4 s[RT][2];  // 32 keys x rows
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -198,122 +367,44 @@ __global__ __launch_bounds__(256) void k_tree_attn(TreeP P) {
 #pragma unroll
           for (int n = NS - 1; n >= 0; --n) s[rt][t] = mfma16(kr[t][ks], q[rt][ks][n], s[rt][t]);
       }
-    const uint32_t present = (uint32_t)(__ballot(ok[0]) & 0xFFFF) | (uint32_t)((__ballot(ok[1]) & 0xFFFF) << 16);
     const bool drafted = kt + 32 > L.ctx;  // the tile reaches the drafted keys or the end
-    const bool masked = present != 0xFFFFFFFFu || drafted;
-    bool bad = false;
-    if (masked) {
-      // an absent key's value is zero; an infinity or NaN in a drafted key's value must not reach the rows that do not see
-      // that key (0 * inf), so it leaves the tile and is added to the others alone
+    if (drafted || present != 0xFFFFFFFFu) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t) {
+        const bool gone = !((present >> (16 * t + r16)) & 1);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          if (!ok[t])
-#pragma unroll
-            for (int i = 0; i < 8; ++i) vr[t][ks][i] = (T)0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t u = __builtin_bit_cast(uint16_t, (T)vr[t][ks][i]);
-            if (drafted && (u & kExp<T>) == kExp<T>) {
-              bad = true;
-              vr[t][ks][i] = (T)0.f;
-            }
-          }
+          if (gone) vr[t][ks] = V8{};  // whatever lies there must not meet a weight of 0
+          if (drafted) bad |= strip_nonfinite<T>(vr[t][ks]);
         }
-      bad = __any(bad);
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) apply_mask(seen_bits(P, w.b, L.ctx, kt, present, node[rt], g4), s[rt]);
     }
-    // V to LDS
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int key = 16 * t + r16, cidx = g4 + 4 * ks;
-        const int pair = (cidx >> 1) ^ (key & (MT >= 8 ? 7 : MT - 1));
-        *reinterpret_cast<V8*>(vl + key * DP + 16 * pair + 8 * (cidx & 1)) = vr[t][ks];
+        const int key = 16 * t + r16;
+        *reinterpret_cast<V8*>(vl + key * DP + 8 * ((g4 + 4 * ks) ^ (key & (PIECES - 1)))) = vr[t][ks];
       }
-    // the next tile's loads go out before the softmax
-    if (kt + 128 < k1) {
+    if (kt + 128 < k1) {  // the next tile's loads go out before the softmax
       issue(kt + 128, pid);
       page_ids(kt + 256, pid);
-    }
-    if (masked) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const uint8_t* mrow = a.mask ? a.mask + b * a.mask_seq + node[rt] * a.mask_row : nullptr;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int kk = 16 * t + 4 * g4 + i, j = kt + kk - L.ctx;
-            bool seen = (present >> kk) & 1;
-            if (seen && j >= 0) seen = mrow ? mrow[j] != 0 : j <= node[rt];
-            if (!seen) s[rt][t][i] = -INFINITY;
-          }
-      }
     }
     V8 p[RT][NS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float top = s[rt][0][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[rt][i >> 2][i & 3]);
-      top = fmaxf(m[rt], across_max(top));
-      const float base = top == -INFINITY ? 0.f : top;  // nothing seen so far: every weight is exp2(-inf) = 0
-      const float alpha = exp2f((m[rt] - base) * P.c);
-      m[rt] = top;
-      float e[8], sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        e[i] = exp2f((s[rt][i >> 2][i & 3] - base) * P.c);
-        sum += e[i];
-      }
-      l[rt] = l[rt] * alpha + sum;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) o[rt][mt] *= alpha;
-      if (bad) {
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = kt + 16 * (i >> 2) + 4 * g + (i & 3);
-            const float w = __shfl(e[i], 16 * g + r16);
-            if (key >= k1) continue;
-            const uint32_t pg = P.page_div.div((uint32_t)key);
-            const int id = table[pg];
-            if (id < 0 || id >= a.pages) continue;
-            const T* vp = vbase + id * a.v_page + (int64_t)((uint32_t)key - pg * a.page_size) * a.v_slot;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int d = 16 * mt + 4 * g4 + j;
-                const float x = d < D ? (float)vp[d] : 0.f;
-                if (!(fabsf(x) < INFINITY) && w != 0.f) o[rt][mt][j] += w * x;
-              }
-          }
-      }
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const T y = (T)e[i];
-          p[rt][n][i] = y;
-          e[i] -= (float)y;
-        }
+      float e[8];
+      softmax_step<MT>(s[rt], P.c, m[rt], l[rt], o[rt], e);
+      to_terms<T, NS>(e, p[rt]);
     }
-    // O^T += V^T P^T
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      V8 v;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int key = 16 * t + 4 * g4 + (r16 >> 2);
-        const int pair = mt ^ (key & (MT >= 8 ? 7 : MT - 1));
-        const v4i16 x = ld_tr(vl + key * DP + 16 * pair + 4 * (r16 & 3));
-        const auto y = __builtin_bit_cast(T __attribute__((ext_vector_type(4))), x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * t + i] = y[i];
-      }
+      const int key = 4 * g4 + (r16 >> 2), piece = 2 * mt + ((r16 >> 1) & 1);
+      const T* const at = vl + key * DP + 8 * (piece ^ (key & (PIECES - 1))) + 4 * (r16 & 1);
+      const T* const at2 = vl + (key + 16) * DP + 8 * (piece ^ ((key + 16) & (PIECES - 1))) + 4 * (r16 & 1);
+      const V8 v = values_operand<T>(at, at2);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -321,9 +412,14 @@ __global__ __launch_bounds__(256) void k_tree_attn(TreeP P) {
     }
   }
 
+  if (__any(bad))
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+      add_nonfinite<T, NS, DP>(P, w, L, k0 + 32 * wave, k1, 128, node[rt], q[rt], m[rt], reinterpret_cast<float*>(vl), o[rt]);
+
   // the four waves' results join through LDS
-  float* const lo = reinterpret_cast<float*>(smem);                 // [4][ROWS][OS]
-  float* const lml = lo + 4 * ROWS * OS;                            // [4][ROWS][2]
+  float* const lo = reinterpret_cast<float*>(smem);  // [4][ROWS][OS]
+  float* const lml = lo + 4 * ROWS * OS;             // [4][ROWS][2]
   __syncthreads();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -343,37 +439,194 @@ __global__ __launch_bounds__(256) void k_tree_attn(TreeP P) {
     if (rr >= rows || e >= D) continue;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, lml[(w * ROWS + row) * 2]);
-    const float base = top == -INFINITY ? 0.f : top;
+    for (int v = 0; v < 4; ++v) top = fmaxf(top, lml[(v * ROWS + row) * 2]);
+    const float base = (top == -INFINITY ? 0.f : top) * P.c;
     float sum = 0.f;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = exp2f((lml[(w * ROWS + row) * 2] - base) * P.c);
-      sum += f * lml[(w * ROWS + row) * 2 + 1];
-      x += f * *reinterpret_cast<const f32x4*>(lo + (w * ROWS + row) * OS + e);
+    for (int v = 0; v < 4; ++v) {
+      const float f = exp2_fast(lml[(v * ROWS + row) * 2] * P.c - base);
+      sum += f * lml[(v * ROWS + row) * 2 + 1];
+      x += f * *reinterpret_cast<const f32x4*>(lo + (v * ROWS + row) * OS + e);
     }
     if (L.splits > 1) {
-      const int64_t at = (((int64_t)b * a.kv_heads + h) * P.splits + split) * P.rows + rr;
+      const int64_t at = (((int64_t)w.b * a.kv_heads + w.h) * P.splits + w.split) * P.rows + rr;
       *reinterpret_cast<f32x4*>(P.part_o + at * DP + e) = x;
-      if (e == 0) {
-        P.part_ml[at * 2] = top;
-        P.part_ml[at * 2 + 1] = sum;
-      }
+      if (e == 0) *reinterpret_cast<float2*>(P.part_ml + at * 2) = make_float2(top, sum);
     } else {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const int nd = (int)P.group_div.div((uint32_t)rr);
-      const int64_t at = b * a.out_seq + nd * a.out_node + (int64_t)(h * P.group + rr - nd * P.group) * a.out_head + e;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (NS > 1) reinterpret_cast<float*>(a.out)[at + i] = x[i] * inv;
-        else reinterpret_cast<T*>(a.out)[at + i] = (T)(x[i] * inv);
-      }
+      const int64_t at = w.b * a.out_seq + nd * a.out_node + (int64_t)(w.h * P.group + rr - nd * P.group) * a.out_head + e;
+      typedef typename std::conditional<(NS > 1), float, T>::type TO;
+      store4(reinterpret_cast<TO*>(a.out) + at, x * (sum == 0.f ? 0.f : 1.f / sum), D - e);
     }
   }
 }
 
-// joins the partial results of a row: a wave a row, lanes over the dimensions
+// KT keys a tile
+template <typename T, int NS, int DP, int RT, int KT>
+__global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_many(TreeP P) {
+  typedef typename Vec8<T>::type V8;
+  constexpr int KS = DP / 32, MT = DP / 16, ROWS = 64 * RT, PIECES = DP / 8, KG = KT / 32;
+  constexpr int NL = KT * PIECES / 256;  // pieces of K (and of V) a thread stages
+  constexpr int KPS = 256 / PIECES;      // keys staged by one piece of every thread
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* const lds = reinterpret_cast<T*>(smem);  // [stage][K, V][KT][DP]
+  const fa_tree_attention_args& a = P.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g4 = lane >> 4;
+  Where w;
+  if (!locate(P, w)) return;
+  const SeqLens L = seq_lens(P, w.b);
+  const int rows = L.n * P.group, r0 = w.q_tile * ROWS;
+  if (r0 >= rows || w.split >= L.splits) return;
+  const int D = a.head_dim;
+  const int k0 = w.split * P.chunk, k1 = w.split == L.splits - 1 ? L.total : min(L.total, k0 + P.chunk);
+  const T* const kbase = reinterpret_cast<const T*>(a.k_cache) + w.h * a.k_head;
+  const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + w.h * a.v_head;
+  const int32_t* const table = a.block_table + w.b * a.table_seq;
+
+  // lane i holds the page number of key kt + i (-1: none)
+  auto page_id = [&](int kt) -> int {
+    const int key = kt + (lane & (KT - 1));
+    const int id = key < k1 ? table[P.page_div.div((uint32_t)key)] : -1;
+    return (uint32_t)id < (uint32_t)a.pages ? id : -1;
+  };
+  V8 kr[NL], vr[NL];
+  const int piece = tid & (PIECES - 1), ec = 8 * piece < D ? 8 * piece : 0;
+  auto issue = [&](int kt, int pid) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int k = i * KPS + tid / PIECES;
+      const uint32_t key = (uint32_t)(kt + k);
+      const int id = __shfl(pid, k), page = max(id, 0);
+      const int off = id < 0 ? 0 : (int)(key - P.page_div.div(key) * a.page_size);
+      kr[i] = *reinterpret_cast<const V8*>(kbase + page * a.k_page + off * a.k_slot + ec);
+      vr[i] = *reinterpret_cast<const V8*>(vbase + page * a.v_page + off * a.v_slot + ec);
+    }
+  };
+  int pid = -1, next = -1;
+  if (k0 < k1) {
+    pid = page_id(k0);
+    issue(k0, pid);
+    next = page_id(k0 + KT);
+  }
+
+  int node[RT];
+  V8 q[RT][KS][NS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) node[rt] = load_q<T, NS, KS>(P, w, r0 + (wave * RT + rt) * 16 + r16, rows, g4, q[rt]);
+  float m[RT], l[RT];
+  f32x4 o[RT][MT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) o[rt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  int stage = 0;
+  bool bad = false;
+  for (int kt = k0; kt < k1; kt += KT, stage ^= 1) {
+    T* const lk = lds + stage * 2 * KT * DP;
+    T* const lv = lk + KT * DP;
+    const uint64_t present = __ballot(pid >= 0) & (KT == 64 ? ~0ull : (1ull << KT) - 1);
+    const bool drafted = kt + KT > L.ctx;
+    const bool masked = drafted || present != (KT == 64 ? ~0ull : (1ull << KT) - 1);
+    uint32_t bits[RT][KG];
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        if (!((present >> (i * KPS + tid / PIECES)) & 1)) vr[i] = V8{};
+        if (drafted) bad |= strip_nonfinite<T>(vr[i]);
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+          bits[rt][g] = seen_bits(P, w.b, L.ctx, kt + 32 * g, (uint32_t)(present >> (32 * g)), node[rt], g4);
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int k = i * KPS + tid / PIECES, at = k * DP + 8 * (piece ^ (k & (PIECES - 1)));
+      *reinterpret_cast<V8*>(lk + at) = kr[i];
+      *reinterpret_cast<V8*>(lv + at) = vr[i];
+    }
+    pid = next;
+    if (kt + KT < k1) {
+      issue(kt + KT, pid);
+      next = page_id(kt + 2 * KT);
+    }
+    // one barrier a tile: a wave writes this stage again two tiles on, behind the barrier at which all have left it
+    __syncthreads();
+
+    f32x4 s[RT][KG][2];
+#pragma unroll
+    for (int g = 0; g < KG; ++g)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int key = 32 * g + 16 * t + r16;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const V8 k = *reinterpret_cast<const V8*>(lk + key * DP + 8 * ((g4 + 4 * ks) ^ (key & (PIECES - 1))));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int n = NS - 1; n >= 0; --n) s[rt][g][t] = mfma16(k, q[rt][ks][n], s[rt][g][t]);
+        }
+      }
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+      V8 p[RT][NS];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        if (masked) apply_mask(bits[rt][g], s[rt][g]);
+        float e[8];
+        softmax_step<MT>(s[rt][g], P.c, m[rt], l[rt], o[rt], e);
+        to_terms<T, NS>(e, p[rt]);
+      }
+  #pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int key = 32 * g + 4 * g4 + (r16 >> 2), pc = 2 * mt + ((r16 >> 1) & 1);
+        const T* const at = lv + key * DP + 8 * (pc ^ (key & (PIECES - 1))) + 4 * (r16 & 1);
+        const T* const at2 = lv + (key + 16) * DP + 8 * (pc ^ ((key + 16) & (PIECES - 1))) + 4 * (r16 & 1);
+        const V8 v = values_operand<T>(at, at2);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int n = NS - 1; n >= 0; --n) o[rt][mt] = mfma16(v, p[rt][n], o[rt][mt]);
+      }
+    }
+  }
+
+  if (__syncthreads_or(bad))
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+      add_nonfinite<T, NS, DP>(P, w, L, k0, k1, 32, node[rt], q[rt], m[rt], reinterpret_cast<float*>(smem) + wave * 512, o[rt]);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int rr = r0 + (wave * RT + rt) * 16 + r16;
+    const float sum = across_sum(l[rt]);
+    if (rr >= rows) continue;
+    if (L.splits > 1) {
+      const int64_t at = (((int64_t)w.b * a.kv_heads + w.h) * P.splits + w.split) * P.rows + rr;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        if (16 * mt + 4 * g4 < D) *reinterpret_cast<f32x4*>(P.part_o + at * DP + 16 * mt + 4 * g4) = o[rt][mt];
+      if (g4 == 0) *reinterpret_cast<float2*>(P.part_ml + at * 2) = make_float2(m[rt], sum);
+    } else {
+      typedef typename std::conditional<(NS > 1), float, T>::type TO;
+      TO* const out = reinterpret_cast<TO*>(a.out) + w.b * a.out_seq + node[rt] * a.out_node +
+                      (int64_t)(w.h * P.group + rr - node[rt] * P.group) * a.out_head;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) store4(out + 16 * mt + 4 * g4, o[rt][mt] * inv, D - 16 * mt - 4 * g4);
+    }
+  }
+}
+
+// joins the partial results of a row: a wave a row; lane s weighs split s (at most 64), then the lanes go over the dimensions
 template <typename TO, int DP>
 __global__ __launch_bounds__(256) void k_tree_merge(TreeP P) {
   const fa_tree_attention_args& a = P.a;
@@ -381,31 +634,35 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeP P) {
   const SeqLens L = seq_lens(P, b);
   if (rr >= L.n * P.group || L.splits == 1) return;
   const int64_t at0 = ((int64_t)b * a.kv_heads + h) * P.splits * P.rows + rr;
-  float top = -INFINITY;
-  for (int s = 0; s < L.splits; ++s) top = fmaxf(top, P.part_ml[(at0 + (int64_t)s * P.rows) * 2]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, x[DP / 64] = {};
-  for (int s = 0; s < L.splits; ++s) {
-    const int64_t at = at0 + (int64_t)s * P.rows;
-    const float f = exp2f((P.part_ml[at * 2] - base) * P.c);
-    sum += f * P.part_ml[at * 2 + 1];
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < L.splits) ml = *reinterpret_cast<const float2*>(P.part_ml + (at0 + (int64_t)lane * P.rows) * 2);
+  const float top = wave_max(ml.x), base = (top == -INFINITY ? 0.f : top) * P.c;
+  float f = exp2_fast(ml.x * P.c - base);
+  const float sum = wave_sum(f * ml.y);
+  f *= sum == 0.f ? 0.f : 1.f / sum;
+  constexpr int N = DP / 64;
+  float x[N] = {};
+  const float* const o = P.part_o + at0 * DP + lane * N;
+  if (lane * N < a.head_dim)
+#pragma unroll 4
+    for (int s = 0; s < L.splits; ++s) {
+      const float g = __shfl(f, s);
 #pragma unroll
-    for (int i = 0; i < DP / 64; ++i)
-      if (lane + 64 * i < a.head_dim) x[i] += f * P.part_o[at * DP + lane + 64 * i];
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      for (int i = 0; i < N; ++i) x[i] += g * o[(int64_t)s * P.rows * DP + i];
+    }
   const int nd = (int)P.group_div.div((uint32_t)rr);
   TO* out = reinterpret_cast<TO*>(a.out) + b * a.out_seq + nd * a.out_node +
-            (int64_t)(h * P.group + rr - nd * P.group) * a.out_head;
+            (int64_t)(h * P.group + rr - nd * P.group) * a.out_head + lane * N;
 #pragma unroll
-  for (int i = 0; i < DP / 64; ++i)
-    if (lane + 64 * i < a.head_dim) out[lane + 64 * i] = (TO)(x[i] * inv);
+  for (int i = 0; i < N; ++i)
+    if (lane * N + i < a.head_dim) out[i] = (TO)x[i];
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
 struct TreePlan {
   TreeP P;
   int dp, rt;
+  bool many;
   int64_t bytes;
 };
 
@@ -432,9 +689,11 @@ static TreePlan tree_plan(const fa_tree_attention_args* ap) {
   t.P.page_div = FastDiv::of((uint32_t)a.page_size);
   t.P.group_div = FastDiv::of((uint32_t)group);
   t.dp = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
-  t.rt = t.dp == 256 || t.P.rows <= 16 ? 1 : 2;
-  t.P.q_tiles = (t.P.rows + 16 * t.rt - 1) / (16 * t.rt);
-  FA_REQUIRE((int64_t)t.P.q_tiles * a.kv_heads <= 65535, "tree_attention: too many rows");
+  // up to 32 rows: k_few; more: k_many, 64 rows a block, or 128 where there are as many and registers allow
+  t.many = t.P.rows > 32 || (t.dp == 256 && t.P.rows > 16);
+  t.rt = t.many ? (t.P.rows > 64 && t.dp <= 128 && a.q_type != FA_F32 ? 2 : 1) : t.P.rows <= 16 ? 1 : 2;
+  const int rows_block = t.many ? 64 * t.rt : 16 * t.rt;
+  t.P.q_tiles = (t.P.rows + rows_block - 1) / rows_block;
   t.bytes = 0;
   t.P.splits = 1;
   t.P.chunk = 1 << 30;
@@ -443,37 +702,65 @@ static TreePlan tree_plan(const fa_tree_attention_args* ap) {
   const int64_t cap = (int64_t)a.table_len * a.page_size;
   const int64_t keys = std::max<int64_t>(1, std::min<int64_t>(cap, a.max_context > 0 ? (int64_t)a.max_context + a.nodes : cap));
   const int64_t base = (int64_t)a.seqs * a.kv_heads * t.P.q_tiles;
-  const int64_t want = std::max<int64_t>(1, (4ll * cu_count() + base - 1) / base);
+  const int64_t want = std::min<int64_t>(64, std::max<int64_t>(1, (4ll * cu_count() + base - 1) / base));
   int64_t chunk = std::max<int64_t>(256, (keys + want - 1) / want);
   chunk = (chunk + 127) / 128 * 128;
   t.P.chunk = (int)chunk;
   t.P.splits = (int)((keys + chunk - 1) / chunk);
+  t.P.q_tiles_div = FastDiv::of((uint32_t)std::max(1, t.P.q_tiles));
+  t.P.kv_div = FastDiv::of((uint32_t)a.kv_heads);
+  t.P.splits_div = FastDiv::of((uint32_t)t.P.splits);
+  const int64_t groups = (int64_t)a.seqs * a.kv_heads * t.P.splits;
+  FA_REQUIRE((groups + 7) / 8 * 8 * t.P.q_tiles < (1ll << 31), "tree_attention: more than 2^31 blocks");
+  t.P.n_groups = (int)groups;
   if (t.P.splits > 1)
     t.bytes = (int64_t)a.seqs * a.kv_heads * t.P.splits * t.P.rows * (t.dp + 2) * (int64_t)sizeof(float);
   return t;
 }
 
-template <typename T, int NS, int DP, int RT>
-static void tree_run(const TreeP& P, hipStream_t s) {
-  constexpr int ROWS = 16 * RT;
-  constexpr size_t lds = std::max<size_t>(4 * 32 * DP * 2, 4 * ROWS * (DP + 4) * 4 + 4 * ROWS * 2 * 4);
-  const fa_tree_attention_args& a = P.a;
-  if constexpr (lds > 65536) {
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k_tree_attn<T, NS, DP, RT>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+// a kernel's LDS beyond 64 KB has to be asked for, once
+template <auto KERNEL, size_t LDS>
+static void tree_launch(const TreeP& P, hipStream_t s) {
+  if constexpr (LDS > 65536) {
+    static const hipError_t once =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
     FA_HIP(once);
   }
-  launch(k_tree_attn<T, NS, DP, RT>, dim3(P.splits, a.kv_heads * P.q_tiles, a.seqs), dim3(256), lds, s, P);
-  if (P.splits > 1) {
+  launch(KERNEL, dim3((uint32_t)((P.n_groups + 7) / 8 * 8) * P.q_tiles), dim3(256), LDS, s, P);
+}
+template <typename T, int NS, int DP, int RT>
+static void run_few(const TreeP& P, hipStream_t s) {
+  constexpr int ROWS = 16 * RT;
+  constexpr size_t lds = std::max<size_t>(4 * 32 * DP * 2, 4 * ROWS * (DP + 4) * 4 + 4 * ROWS * 2 * 4);
+  P.a.head_dim == DP ? tree_launch<k_few<T, NS, DP, RT, true>, lds>(P, s) : tree_launch<k_few<T, NS, DP, RT, false>, lds>(P, s);
+}
+template <typename T, int NS, int DP, int RT>
+static void run_many(const TreeP& P, hipStream_t s) {
+  constexpr int KT = DP == 256 ? 32 : 64;
+  constexpr size_t lds = 4 * KT * DP * 2;  // two stages of K and V
+  tree_launch<k_many<T, NS, DP, RT, KT>, lds>(P, s);
+}
+template <typename T, int NS, int DP>
+static void tree_run(const TreePlan& t, hipStream_t s) {
+  if constexpr (DP == 256) {
+    t.many ? run_many<T, NS, 256, 1>(t.P, s) : run_few<T, NS, 256, 1>(t.P, s);
+  } else if (!t.many) {
+    t.rt == 1 ? run_few<T, NS, DP, 1>(t.P, s) : run_few<T, NS, DP, 2>(t.P, s);
+  } else if constexpr (NS == 1) {
+    t.rt == 1 ? run_many<T, NS, DP, 1>(t.P, s) : run_many<T, NS, DP, 2>(t.P, s);
+  } else {
+    run_many<T, NS, DP, 1>(t.P, s);
+  }
+  if (t.P.splits > 1) {
     typedef typename std::conditional<(NS > 1), float, T>::type TO;
-    launch(k_tree_merge<TO, DP>, dim3((P.rows + 3) / 4, a.kv_heads, a.seqs), dim3(256), 0, s, P);
+    launch(k_tree_merge<TO, DP>, dim3((t.P.rows + 3) / 4, t.P.a.kv_heads, t.P.a.seqs), dim3(256), 0, s, t.P);
   }
 }
 template <typename T, int NS>
 static void tree_dispatch(const TreePlan& t, hipStream_t s) {
-  if (t.dp == 64) t.rt == 1 ? tree_run<T, NS, 64, 1>(t.P, s) : tree_run<T, NS, 64, 2>(t.P, s);
-  else if (t.dp == 128) t.rt == 1 ? tree_run<T, NS, 128, 1>(t.P, s) : tree_run<T, NS, 128, 2>(t.P, s);
-  else tree_run<T, NS, 256, 1>(t.P, s);
+  if (t.dp == 64) tree_run<T, NS, 64>(t, s);
+  else if (t.dp == 128) tree_run<T, NS, 128>(t, s);
+  else tree_run<T, NS, 256>(t, s);
 }
 
 static void tree_attention(const fa_tree_attention_args* ap, hipStream_t s) {
@@ -488,7 +775,6 @@ static void tree_attention(const fa_tree_attention_args* ap, hipStream_t s) {
              "tree_attention: workspace too small or not 16-byte aligned");
   const int64_t qm = 16 / type_bytes(a.q_type);
   t.P.q_vec = aligned16(a.q) && a.q_seq % qm == 0 && a.q_node % qm == 0 && a.q_head % qm == 0;
-  t.P.out_vec = 0;
   t.P.part_o = reinterpret_cast<float*>(a.workspace);
   t.P.part_ml = t.P.part_o + (int64_t)a.seqs * a.kv_heads * t.P.splits * t.P.rows * t.dp;
   if (a.cache_type == FA_F16) {
