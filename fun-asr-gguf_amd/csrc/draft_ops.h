@@ -45,20 +45,19 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 }
 
 // x / d for 0 <= x < 2^31 and a divisor 1 <= d < 2^31 that only the host knows beforehand: with s = ceil(log2 d) and
-// m = floor(2^(31 + s) / d) + 1 <= 2^32, x m / 2^(31 + s) exceeds x / d by at most x / 2^(31 + s) < 1 / d, so the floors agree.
+// m = floor(2^32 (2^s - d) / d) + 1 < 2^32, (2^32 + m) x / 2^(32 + s) exceeds x / d by less than x / 2^(32 + s) < 1 / d, so
+// the floors agree; the high half of m x plus x stays below 2^32.
 struct FastDiv {
-  uint64_t mul = 0;
-  uint32_t shift = 0, d = 1;
+  uint32_t mul = 1, shift = 0;
   static FastDiv of(uint32_t d) {
     FastDiv f;
-    f.d = d;
-    uint32_t s = 0;
-    while ((1ull << s) < d) ++s;
-    f.shift = 31 + s;
-    f.mul = (1ull << f.shift) / d + 1;
+    while ((1ull << f.shift) < d) ++f.shift;
+    f.mul = (uint32_t)((1ull << 32) * ((1ull << f.shift) - d) / d + 1);
     return f;
   }
-  __host__ __device__ __forceinline__ uint32_t div(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
+  __host__ __device__ __forceinline__ uint32_t div(uint32_t x) const {
+    return ((uint32_t)(((uint64_t)x * mul) >> 32) + x) >> shift;
+  }
 };
 
 inline int type_bytes(int t) { return t == FA_F32 ? 4 : 2; }

@@ -41,6 +41,9 @@ struct TreeP {
   float* part_o;       // [seqs][kv_heads][splits][rows][DP]
   float* part_ml;      // [seqs][kv_heads][splits][rows][2]
   int q_vec;           // q's rows may be read in 16-byte pieces
+  uint32_t k_page, k_slot, v_page, v_slot;  // strides, below 2^31 (checked by the host): one multiply-add a product
+  int one_offset;      // K's and V's strides are the same
+  int uniform;         // so many consecutive keys, or a divisor of it, lie in one page: page_size, or 1 (see UNI)
 };
 
 __device__ __forceinline__ f32x4 mfma16(f16x8_t a, f16x8_t b, f32x4 c) {
@@ -51,10 +54,13 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8_t a, bf16x8_t b, f32x4 c) {
 }
 // 2^x; results below 2^-126 become 0 (weights that far under the row's largest)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// over the four 16-lane groups of a wave
+// over the four 16-lane groups of a wave: a swap of a register with itself leaves one half (or one 16-lane row of each pair)
+// twice in the first and the other twice in the second
 __device__ __forceinline__ float across_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float across_sum(float v) {
   v += __shfl_xor(v, 16);
@@ -69,10 +75,10 @@ struct SeqLens {
 };
 __device__ __forceinline__ SeqLens seq_lens(const TreeP& P, int b) {
   const fa_tree_attention_args& a = P.a;
-  SeqLens s;
-  s.n = a.draft_lens ? min(max(a.draft_lens[b], 0), a.nodes) : a.nodes;
+  SeqLens s;  // (kept in scalar registers, and what follows from them)
+  s.n = a.draft_lens ? min(max(__builtin_amdgcn_readfirstlane(a.draft_lens[b]), 0), a.nodes) : a.nodes;
   const int cap = a.table_len * a.page_size;  // < 2^31 - nodes (checked by the host)
-  s.ctx = min(max(a.context_lens[b], 0), cap);
+  s.ctx = min(max(__builtin_amdgcn_readfirstlane(a.context_lens[b]), 0), cap);
   s.total = min(s.ctx + s.n, cap);
   s.splits = min(P.splits, max(1, (s.total + P.chunk - 1) / P.chunk));
   return s;
@@ -133,49 +139,78 @@ __device__ __forceinline__ int load_q(const TreeP& P, const Where& w, int rr, in
 // present: the group's keys that exist
 __device__ __forceinline__ uint32_t seen_bits(const TreeP& P, int b, int ctx, int kt, uint32_t present, int node, int g4) {
   const fa_tree_attention_args& a = P.a;
+  // the drafted keys' part: eight loads at once, or the order of the tokens; in integers (conditions would take two scalar
+  // registers each)
+  const int j0 = kt + 4 * g4 - ctx;
+  uint32_t drafted[8];
+  if (a.mask) {
+    const uint8_t* const row = a.mask + b * a.mask_seq + node * a.mask_row;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) drafted[i] = row[min(max(j0 + 16 * (i >> 2) + (i & 3), 0), a.nodes - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) drafted[i] = min(drafted[i], 1u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) drafted[i] = (uint32_t)(j0 + 16 * (i >> 2) + (i & 3) - node - 1) >> 31;
+  }
+  present >>= 4 * g4;
   uint32_t bits = 0;
-  const uint8_t* const row = a.mask ? a.mask + b * a.mask_seq + node * a.mask_row : nullptr;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int kk = 16 * (i >> 2) + 4 * g4 + (i & 3), j = kt + kk - ctx;
-    const uint32_t drafted = row ? row[min(max(j, 0), a.nodes - 1)] != 0 : j <= node;
-    bits |= ((present >> kk) & (j < 0 ? 1u : drafted) & 1u) << i;
+    const int kk = 16 * (i >> 2) + (i & 3);
+    bits |= ((present >> kk) & (drafted[i] | (uint32_t)(j0 + kk) >> 31) & 1u) << i;
   }
   return bits;
 }
 
-// One group of 32 keys of the softmax: scores s -> weights e relative to the running maximum; o and l rescaled
-template <int MT>
-__device__ __forceinline__ void softmax_step(const f32x4 (&s)[2], float c, float& m, float& l, f32x4 (&o)[MT], float (&e)[8]) {
-  float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                    fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-  top = fmaxf(m, across_max(top));
+// KG groups of 32 keys of the softmax: scores s -> weights in their place, relative to the running maximum; o and l rescaled
+template <int MT, int KG>
+__device__ __forceinline__ void softmax_step(f32x4 (&s)[KG][2], float c, float& m, float& l, f32x4 (&o)[MT]) {
+  float top = m;
+#pragma unroll
+  for (int g = 0; g < KG; ++g)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) top = fmaxf(top, fmaxf(fmaxf(s[g][t][0], s[g][t][1]), fmaxf(s[g][t][2], s[g][t][3])));
+  top = across_max(top);
   const float base = (top == -INFINITY ? 0.f : top) * c;  // nothing seen so far: every weight is 2^-inf = 0
-  const float alpha = exp2_fast(m * c - base);
-  if (__any(top != m)) {  // (first tiles mostly)
+  if (__any(top != m)) {                                  // (first tiles mostly)
+    const float alpha = exp2_fast(m * c - base);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) o[mt] *= alpha;
     l *= alpha;
   }
   m = top;
-  float sum = 0.f;
+  float sum[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    e[i] = exp2_fast(fmaf(s[i >> 2][i & 3], c, -base));
-    sum += e[i];
-  }
-  l += sum;
+  for (int g = 0; g < KG; ++g)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = exp2_fast(fmaf(s[g][t][i], c, -base));
+        s[g][t][i] = e;
+        sum[t] += e;
+      }
+  l += sum[0] + sum[1];
 }
 template <typename T, int NS>
-__device__ __forceinline__ void to_terms(float (&e)[8], typename Vec8<T>::type (&p)[NS]) {
+__device__ __forceinline__ void to_terms(const f32x4 (&s)[2], typename Vec8<T>::type (&p)[NS]) {
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
+  for (int i = 0; i < 8; ++i) {
+    float e = s[i >> 2][i & 3];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const T y = (T)e[i];
+    for (int n = 0; n < NS; ++n) {
+      const T y = (T)e;
       p[n][i] = y;
-      e[i] -= (float)y;
+      e -= (float)y;
     }
+  }
+}
+
+// eight elements at p + i. As a 32-bit offset in bytes under the pointer: where that is a scalar, the load adds them itself
+template <typename T>
+__device__ __forceinline__ typename Vec8<T>::type piece_at(const T* p, uint32_t i) {
+  return *reinterpret_cast<const typename Vec8<T>::type*>(reinterpret_cast<const char*>(p) + i * 2u);
 }
 
 // sets the infinities and NaN among 8 values to 0; true if there were any
@@ -283,14 +318,16 @@ __device__ __forceinline__ void store4(TO* p, f32x4 x, int left) {
 // 24 bits by terms of float16 / bfloat16; with 1 term the weights are rounded to the cache's type, half a step of it, as the
 // output is). DP: head_dim rounded up to 64 / 128 / 256. FULL: it is DP itself; else a piece behind head_dim is read at 0
 // instead (q is 0 there, and the output's dimensions behind it are not written).
-template <typename T, int NS, int DP, int RT, bool FULL>
-__global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_few(TreeP P) {
+// UNI: 16 consecutive keys from a multiple of 16 on lie in one page (page_size is a multiple of 16), so a page's address is a
+// scalar and a lane's place under it a constant 32-bit offset; else every lane looks up its own keys' pages.
+template <typename T, int NS, int DP, int RT, bool FULL, bool UNI>
+__global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void k_few(TreeP P) {
   typedef typename Vec8<T>::type V8;
   constexpr int KS = DP / 32, MT = DP / 16, ROWS = 16 * RT, PIECES = DP / 8;
   constexpr int OS = DP + 4;  // output rows in LDS: 16 rows of a float4 store on different banks
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const fa_tree_attention_args& a = P.a;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g4 = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g4 = lane >> 4;
   Where w;
   if (!locate(P, w)) return;
   const SeqLens L = seq_lens(P, w.b);
@@ -303,41 +340,54 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_few(T
   const int32_t* const table = a.block_table + w.b * a.table_seq;
   T* const vl = reinterpret_cast<T*>(smem) + wave * 32 * DP;
 
-  // page numbers of this lane's two keys of a tile (16 t + r16): -1 behind the end
-  auto page_ids = [&](int kt, int (&pid)[2]) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int key = kt + 16 * t + r16;
-      pid[t] = key < k1 ? table[P.page_div.div((uint32_t)key)] : -1;
+  // the page numbers a tile needs, -1 behind the end: of this lane's keys 16 t + r16, or of the keys 16 t (lane t). They are
+  // looked at a tile later: nothing waits for their load
+  typedef typename std::conditional<UNI, int, int2>::type Ids;
+  auto page_ids = [&](int kt) -> Ids {
+    if constexpr (UNI) {
+      const int key = kt + 16 * (lane & 1);
+      return key < k1 ? table[P.page_div.div((uint32_t)key)] : -1;
+    } else {
+      const int key = kt + r16;
+      return make_int2(key < k1 ? table[P.page_div.div((uint32_t)key)] : -1,
+                       key + 16 < k1 ? table[P.page_div.div((uint32_t)key + 16)] : -1);
     }
   };
   V8 kr[2][KS], vr[2][KS];
   uint32_t present = 0;
-  // every lane loads: one without a key of its own reads page 0, slot 0 (there is one), which the masks then leave out
-  auto issue = [&](int kt, const int (&pid)[2]) {
-    bool ok[2];
+  const uint32_t klane = UNI ? r16 * P.k_slot : 0, vlane = UNI ? r16 * P.v_slot : 0;
+  // every lane loads: without a page, or behind the end, from page 0 or the page's rest, which the masks then leave out
+  auto issue = [&](int kt, Ids ids) {
+    present = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint32_t key = (uint32_t)(kt + 16 * t + r16);
-      ok[t] = (uint32_t)pid[t] < (uint32_t)a.pages;
-      const int page = ok[t] ? pid[t] : 0, off = ok[t] ? (int)(key - P.page_div.div(key) * a.page_size) : 0;
-      const T* const kp = kbase + page * a.k_page + off * a.k_slot;
-      const T* const vp = vbase + page * a.v_page + off * a.v_slot;
+      const uint32_t key = (uint32_t)(kt + 16 * t) + (UNI ? 0 : r16);
+      int id;
+      if constexpr (UNI) id = __builtin_amdgcn_readlane(ids, t);
+      else id = t ? ids.y : ids.x;
+      const bool ok = (uint32_t)id < (uint32_t)a.pages;
+      const int own = ok ? -1 : 0;  // (all bits)
+      const uint32_t page = id & own, off = (key - P.page_div.div(key) * a.page_size) & own;
+      const uint64_t ko = (uint64_t)page * P.k_page + (uint64_t)off * P.k_slot;
+      const T* const kp = kbase + ko;
+      const T* const vp = vbase + (P.one_offset ? ko : (uint64_t)page * P.v_page + (uint64_t)off * P.v_slot);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const int e = 8 * (g4 + 4 * ks), ec = FULL || e < D ? e : 0;
-        kr[t][ks] = *reinterpret_cast<const V8*>(kp + ec);
-        vr[t][ks] = *reinterpret_cast<const V8*>(vp + ec);
+        const int e = 8 * (g4 + 4 * ks);
+        const uint32_t ec = FULL || e < D ? e : 0;
+        kr[t][ks] = piece_at(kp, klane + ec);
+        vr[t][ks] = piece_at(vp, vlane + ec);
       }
+      if constexpr (UNI) present |= ok ? ((1u << min(max(k1 - (int)key, 0), 16)) - 1) << (16 * t) : 0;
+      else present |= (uint32_t)(__ballot(ok) & 0xFFFF) << (16 * t);
     }
-    present = (uint32_t)(__ballot(ok[0]) & 0xFFFF) | (uint32_t)(__ballot(ok[1]) << 16);
   };
-  int pid[2];
+  Ids ids{};
   int kt = k0 + 32 * wave;
   if (kt < k1) {
-    page_ids(kt, pid);
-    issue(kt, pid);
-    page_ids(kt + 128, pid);
+    ids = page_ids(kt);
+    issue(kt, ids);
+    ids = page_ids(kt + 128);
   }
 
   int node[RT];
@@ -356,17 +406,17 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_few(T
 
   bool bad = false;
   for (; kt < k1; kt += 128) {
-    f32x4 s[RT][2];  // 32 keys x rows
+    f32x4 s[RT][1][2];  // 32 keys x rows
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int rt = 0; rt < RT; ++rt) s[rt][0][0] = s[rt][0][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int ks = 0; ks < KS; ++ks)  // (2 RT sums side by side: a matrix instruction need not wait for the one before it)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+      for (int n = NS - 1; n >= 0; --n)
 #pragma unroll
-          for (int n = NS - 1; n >= 0; --n) s[rt][t] = mfma16(kr[t][ks], q[rt][ks][n], s[rt][t]);
-      }
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][0][t] = mfma16(kr[t][ks], q[rt][ks][n], s[rt][0][t]);
     const bool drafted = kt + 32 > L.ctx;  // the tile reaches the drafted keys or the end
     if (drafted || present != 0xFFFFFFFFu) {
 #pragma unroll
@@ -379,7 +429,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_few(T
         }
       }
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) apply_mask(seen_bits(P, w.b, L.ctx, kt, present, node[rt], g4), s[rt]);
+      for (int rt = 0; rt < RT; ++rt) apply_mask(seen_bits(P, w.b, L.ctx, kt, present, node[rt], g4), s[rt][0]);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -389,15 +439,14 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_few(T
         *reinterpret_cast<V8*>(vl + key * DP + 8 * ((g4 + 4 * ks) ^ (key & (PIECES - 1)))) = vr[t][ks];
       }
     if (kt + 128 < k1) {  // the next tile's loads go out before the softmax
-      issue(kt + 128, pid);
-      page_ids(kt + 256, pid);
+      issue(kt + 128, ids);
+      ids = page_ids(kt + 256);
     }
     V8 p[RT][NS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float e[8];
-      softmax_step<MT>(s[rt], P.c, m[rt], l[rt], o[rt], e);
-      to_terms<T, NS>(e, p[rt]);
+      softmax_step<MT, 1>(s[rt], P.c, m[rt], l[rt], o[rt]);
+      to_terms<T, NS>(s[rt][0], p[rt]);
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -462,9 +511,9 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_few(T
   }
 }
 
-// KT keys a tile
-template <typename T, int NS, int DP, int RT, int KT>
-__global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_many(TreeP P) {
+// KT keys a tile. UNI: KPS consecutive keys from a multiple of KPS on lie in one page
+template <typename T, int NS, int DP, int RT, int KT, bool UNI>
+__global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void k_many(TreeP P) {
   typedef typename Vec8<T>::type V8;
   constexpr int KS = DP / 32, MT = DP / 16, ROWS = 64 * RT, PIECES = DP / 8, KG = KT / 32;
   constexpr int NL = KT * PIECES / 256;  // pieces of K (and of V) a thread stages
@@ -472,7 +521,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_many(
   extern __shared__ __attribute__((aligned(16))) char smem[];
   T* const lds = reinterpret_cast<T*>(smem);  // [stage][K, V][KT][DP]
   const fa_tree_attention_args& a = P.a;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g4 = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g4 = lane >> 4;
   Where w;
   if (!locate(P, w)) return;
   const SeqLens L = seq_lens(P, w.b);
@@ -484,23 +533,35 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_many(
   const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + w.h * a.v_head;
   const int32_t* const table = a.block_table + w.b * a.table_seq;
 
-  // lane i holds the page number of key kt + i (-1: none)
+  // lane i holds the page number of key kt + i, or of key kt + i KPS (-1: none), looked at a tile later: nothing waits for its
+  // load here
   auto page_id = [&](int kt) -> int {
-    const int key = kt + (lane & (KT - 1));
-    const int id = key < k1 ? table[P.page_div.div((uint32_t)key)] : -1;
-    return (uint32_t)id < (uint32_t)a.pages ? id : -1;
+    const int key = kt + (UNI ? KPS * (lane & (NL - 1)) : lane & (KT - 1));
+    return key < k1 ? table[P.page_div.div((uint32_t)key)] : -1;
   };
   V8 kr[NL], vr[NL];
-  const int piece = tid & (PIECES - 1), ec = 8 * piece < D ? 8 * piece : 0;
+  uint64_t arrived = 0, present = 0;  // the keys that exist, of the tile being loaded and of the one at hand
+  const int piece = tid & (PIECES - 1), ec = 8 * piece < D ? 8 * piece : 0, row = tid / PIECES;
+  const uint32_t klane = (UNI ? row * P.k_slot : 0) + ec, vlane = (UNI ? row * P.v_slot : 0) + ec;
   auto issue = [&](int kt, int pid) {
+    if constexpr (UNI) arrived = 0;
+    else arrived = __ballot((uint32_t)pid < (uint32_t)a.pages) & (KT == 64 ? ~0ull : (1ull << KT) - 1);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int k = i * KPS + tid / PIECES;
+      const int k = i * KPS + (UNI ? 0 : row);
       const uint32_t key = (uint32_t)(kt + k);
-      const int id = __shfl(pid, k), page = max(id, 0);
-      const int off = id < 0 ? 0 : (int)(key - P.page_div.div(key) * a.page_size);
-      kr[i] = *reinterpret_cast<const V8*>(kbase + page * a.k_page + off * a.k_slot + ec);
-      vr[i] = *reinterpret_cast<const V8*>(vbase + page * a.v_page + off * a.v_slot + ec);
+      int id;
+      if constexpr (UNI) id = __builtin_amdgcn_readlane(pid, i);
+      else id = __shfl(pid, k);
+      const bool ok = (uint32_t)id < (uint32_t)a.pages;
+      const int own = ok ? -1 : 0;  // (all bits)
+      const uint32_t page = id & own, off = (key - P.page_div.div(key) * a.page_size) & own;
+      const uint64_t ko = (uint64_t)page * P.k_page + (uint64_t)off * P.k_slot;
+      const T* const kp = kbase + ko;
+      const T* const vp = vbase + (P.one_offset ? ko : (uint64_t)page * P.v_page + (uint64_t)off * P.v_slot);
+      kr[i] = piece_at(kp, klane);
+      vr[i] = piece_at(vp, vlane);
+      if constexpr (UNI) arrived |= ok ? ((1ull << min(max(k1 - (int)key, 0), KPS)) - 1) << (i * KPS) : 0;
     }
   };
   int pid = -1, next = -1;
@@ -529,14 +590,14 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_many(
   for (int kt = k0; kt < k1; kt += KT, stage ^= 1) {
     T* const lk = lds + stage * 2 * KT * DP;
     T* const lv = lk + KT * DP;
-    const uint64_t present = __ballot(pid >= 0) & (KT == 64 ? ~0ull : (1ull << KT) - 1);
+    present = arrived;
     const bool drafted = kt + KT > L.ctx;
     const bool masked = drafted || present != (KT == 64 ? ~0ull : (1ull << KT) - 1);
     uint32_t bits[RT][KG];
     if (masked) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        if (!((present >> (i * KPS + tid / PIECES)) & 1)) vr[i] = V8{};
+        if (!((present >> (i * KPS + row)) & 1)) vr[i] = V8{};
         if (drafted) bad |= strip_nonfinite<T>(vr[i]);
       }
 #pragma unroll
@@ -547,7 +608,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_many(
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int k = i * KPS + tid / PIECES, at = k * DP + 8 * (piece ^ (k & (PIECES - 1)));
+      const int k = i * KPS + row, at = k * DP + 8 * (piece ^ (k & (PIECES - 1)));
       *reinterpret_cast<V8*>(lk + at) = kr[i];
       *reinterpret_cast<V8*>(lv + at) = vr[i];
     }
@@ -561,32 +622,34 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 ? 1 : 2) void k_many(
 
     f32x4 s[RT][KG][2];
 #pragma unroll
-    for (int g = 0; g < KG; ++g)
+    for (int g = 0; g < KG; ++g) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int rt = 0; rt < RT; ++rt) s[rt][g][0] = s[rt][g][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const int key = 32 * g + 16 * t + r16;
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+        for (int t = 0; t < 2; ++t) {
+          const int key = 32 * g + 16 * t + r16;
           const V8 k = *reinterpret_cast<const V8*>(lk + key * DP + 8 * ((g4 + 4 * ks) ^ (key & (PIECES - 1))));
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int n = NS - 1; n >= 0; --n) s[rt][g][t] = mfma16(k, q[rt][ks][n], s[rt][g][t]);
         }
-      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (masked)
+#pragma unroll
+        for (int g = 0; g < KG; ++g) apply_mask(bits[rt][g], s[rt][g]);
+      softmax_step<MT, KG>(s[rt], P.c, m[rt], l[rt], o[rt]);
+    }
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
       V8 p[RT][NS];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        if (masked) apply_mask(bits[rt][g], s[rt][g]);
-        float e[8];
-        softmax_step<MT>(s[rt][g], P.c, m[rt], l[rt], o[rt], e);
-        to_terms<T, NS>(e, p[rt]);
-      }
-  #pragma unroll
+      for (int rt = 0; rt < RT; ++rt) to_terms<T, NS>(s[rt][g], p[rt]);
+#pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const int key = 32 * g + 4 * g4 + (r16 >> 2), pc = 2 * mt + ((r16 >> 1) & 1);
         const T* const at = lv + key * DP + 8 * (pc ^ (key & (PIECES - 1))) + 4 * (r16 & 1);
@@ -732,13 +795,19 @@ template <typename T, int NS, int DP, int RT>
 static void run_few(const TreeP& P, hipStream_t s) {
   constexpr int ROWS = 16 * RT;
   constexpr size_t lds = std::max<size_t>(4 * 32 * DP * 2, 4 * ROWS * (DP + 4) * 4 + 4 * ROWS * 2 * 4);
-  P.a.head_dim == DP ? tree_launch<k_few<T, NS, DP, RT, true>, lds>(P, s) : tree_launch<k_few<T, NS, DP, RT, false>, lds>(P, s);
+  const bool full = P.a.head_dim == DP;
+  if (P.uniform % 16 == 0)
+    full ? tree_launch<k_few<T, NS, DP, RT, true, true>, lds>(P, s) : tree_launch<k_few<T, NS, DP, RT, false, true>, lds>(P, s);
+  else
+    tree_launch<k_few<T, NS, DP, RT, false, false>, lds>(P, s);
 }
 template <typename T, int NS, int DP, int RT>
 static void run_many(const TreeP& P, hipStream_t s) {
   constexpr int KT = DP == 256 ? 32 : 64;
   constexpr size_t lds = 4 * KT * DP * 2;  // two stages of K and V
-  tree_launch<k_many<T, NS, DP, RT, KT>, lds>(P, s);
+  constexpr int KPS = 2048 / DP;
+  P.uniform % KPS == 0 ? tree_launch<k_many<T, NS, DP, RT, KT, true>, lds>(P, s)
+                       : tree_launch<k_many<T, NS, DP, RT, KT, false>, lds>(P, s);
 }
 template <typename T, int NS, int DP>
 static void tree_run(const TreePlan& t, hipStream_t s) {
@@ -771,6 +840,15 @@ static void tree_attention(const fa_tree_attention_args* ap, hipStream_t s) {
   FA_REQUIRE(aligned16(a.k_cache) && aligned16(a.v_cache) && a.k_page % 8 == 0 && a.k_head % 8 == 0 && a.k_slot % 8 == 0 &&
                  a.v_page % 8 == 0 && a.v_head % 8 == 0 && a.v_slot % 8 == 0,
              "tree_attention: cache rows must be 16-byte aligned");
+  for (const int64_t x : {a.k_page, a.k_slot, a.v_page, a.v_slot})
+    FA_REQUIRE(x >= 0 && x < (1ll << 31), "tree_attention: a page or slot stride outside 0 .. 2^31");
+  t.P.k_page = (uint32_t)a.k_page;
+  t.P.k_slot = (uint32_t)a.k_slot;
+  t.P.v_page = (uint32_t)a.v_page;
+  t.P.v_slot = (uint32_t)a.v_slot;
+  t.P.one_offset = a.k_page == a.v_page && a.k_slot == a.v_slot;
+  // UNI's offsets of a lane within a page's rows stay below 2^31 bytes
+  t.P.uniform = std::max(a.k_slot, a.v_slot) < (1ll << 24) ? a.page_size : 1;
   FA_REQUIRE(t.bytes == 0 || (a.workspace && a.workspace_bytes >= t.bytes && aligned16(a.workspace)),
              "tree_attention: workspace too small or not 16-byte aligned");
   const int64_t qm = 16 / type_bytes(a.q_type);
