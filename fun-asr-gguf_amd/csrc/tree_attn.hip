@@ -85,14 +85,15 @@ __device__ __forceinline__ SeqLens seq_lens(const TreeP& P, int b) {
 }
 
 // The block's part: consecutive block numbers go round the XCDs, so the row tiles of one (sequence, kv head, split), which
-// read the same keys, are 8 numbers apart: one XCD's L2 fetches those keys once. false: a block of the round-up
+// read the same keys, are 8 numbers apart: one XCD's L2 fetches those keys once. The eight triples of a round turn by one from
+// round to round, else one XCD would get the last (short) splits of all sequences. false: a block of the round-up
 struct Where {
   int b, h, split, q_tile;
 };
 __device__ __forceinline__ bool locate(const TreeP& P, Where& w) {
   const uint32_t xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, g8 = P.q_tiles_div.div(slot);
   w.q_tile = (int)(slot - g8 * P.q_tiles);
-  const uint32_t g = g8 * 8 + xcd;
+  const uint32_t g = g8 * 8 + ((xcd + g8) & 7);
   if (g >= (uint32_t)P.n_groups) return false;
   const uint32_t bh = P.splits_div.div(g);
   w.split = (int)(g - bh * P.splits);
@@ -330,29 +331,26 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g4 = lane >> 4;
   Where w;
   if (!locate(P, w)) return;
-  const SeqLens L = seq_lens(P, w.b);
-  const int rows = L.n * P.group, r0 = w.q_tile * ROWS;
-  if (r0 >= rows || w.split >= L.splits) return;
-  const int D = a.head_dim;
-  const int k0 = w.split * P.chunk, k1 = w.split == L.splits - 1 ? L.total : min(L.total, k0 + P.chunk);
+  const int D = a.head_dim, r0 = w.q_tile * ROWS, k0 = w.split * P.chunk;
   const T* const kbase = reinterpret_cast<const T*>(a.k_cache) + w.h * a.k_head;
   const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + w.h * a.v_head;
   const int32_t* const table = a.block_table + w.b * a.table_seq;
   T* const vl = reinterpret_cast<T*>(smem) + wave * 32 * DP;
 
-  // the page numbers a tile needs, -1 behind the end: of this lane's keys 16 t + r16, or of the keys 16 t (lane t). They are
-  // looked at a tile later: nothing waits for their load
+  // the page numbers a tile needs: of this lane's keys 16 t + r16, or of the keys 16 t (lane t). They are looked at a tile
+  // later: nothing waits for their load; nor does it wait for the lengths (entries behind the end are read, never used)
   typedef typename std::conditional<UNI, int, int2>::type Ids;
   auto page_ids = [&](int kt) -> Ids {
-    if constexpr (UNI) {
-      const int key = kt + 16 * (lane & 1);
-      return key < k1 ? table[P.page_div.div((uint32_t)key)] : -1;
-    } else {
-      const int key = kt + r16;
-      return make_int2(key < k1 ? table[P.page_div.div((uint32_t)key)] : -1,
-                       key + 16 < k1 ? table[P.page_div.div((uint32_t)key + 16)] : -1);
-    }
+    auto entry = [&](int key) { return table[min(P.page_div.div((uint32_t)key), (uint32_t)a.table_len - 1)]; };
+    if constexpr (UNI) return entry(kt + 16 * (lane & 1));
+    else return make_int2(entry(kt + r16), entry(kt + 16 + r16));
   };
+  int kt = k0 + 32 * wave;
+  Ids ids = page_ids(kt);
+  const SeqLens L = seq_lens(P, w.b);
+  const int rows = L.n * P.group;
+  if (r0 >= rows || w.split >= L.splits) return;
+  const int k1 = w.split == L.splits - 1 ? L.total : min(L.total, k0 + P.chunk);
   V8 kr[2][KS], vr[2][KS];
   uint32_t present = 0;
   const uint32_t klane = UNI ? r16 * P.k_slot : 0, vlane = UNI ? r16 * P.v_slot : 0;
@@ -365,7 +363,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
       int id;
       if constexpr (UNI) id = __builtin_amdgcn_readlane(ids, t);
       else id = t ? ids.y : ids.x;
-      const bool ok = (uint32_t)id < (uint32_t)a.pages;
+      const bool ok = (uint32_t)id < (uint32_t)a.pages && (int)key < k1;
       const int own = ok ? -1 : 0;  // (all bits)
       const uint32_t page = id & own, off = (key - P.page_div.div(key) * a.page_size) & own;
       const uint64_t ko = (uint64_t)page * P.k_page + (uint64_t)off * P.k_slot;
@@ -378,14 +376,11 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
         kr[t][ks] = piece_at(kp, klane + ec);
         vr[t][ks] = piece_at(vp, vlane + ec);
       }
-      if constexpr (UNI) present |= ok ? ((1u << min(max(k1 - (int)key, 0), 16)) - 1) << (16 * t) : 0;
+      if constexpr (UNI) present |= ok ? ((1u << min(k1 - (int)key, 16)) - 1) << (16 * t) : 0;
       else present |= (uint32_t)(__ballot(ok) & 0xFFFF) << (16 * t);
     }
   };
-  Ids ids{};
-  int kt = k0 + 32 * wave;
   if (kt < k1) {
-    ids = page_ids(kt);
     issue(kt, ids);
     ids = page_ids(kt + 128);
   }
@@ -524,28 +519,29 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g4 = lane >> 4;
   Where w;
   if (!locate(P, w)) return;
-  const SeqLens L = seq_lens(P, w.b);
-  const int rows = L.n * P.group, r0 = w.q_tile * ROWS;
-  if (r0 >= rows || w.split >= L.splits) return;
-  const int D = a.head_dim;
-  const int k0 = w.split * P.chunk, k1 = w.split == L.splits - 1 ? L.total : min(L.total, k0 + P.chunk);
+  const int D = a.head_dim, r0 = w.q_tile * ROWS, k0 = w.split * P.chunk;
   const T* const kbase = reinterpret_cast<const T*>(a.k_cache) + w.h * a.k_head;
   const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + w.h * a.v_head;
   const int32_t* const table = a.block_table + w.b * a.table_seq;
 
-  // lane i holds the page number of key kt + i, or of key kt + i KPS (-1: none), looked at a tile later: nothing waits for its
-  // load here
+  // lane i holds the page number of key kt + i, or of key kt + i KPS, looked at a tile later: nothing waits for its load here,
+  // nor does it wait for the lengths (entries behind the end are read, never used)
   auto page_id = [&](int kt) -> int {
     const int key = kt + (UNI ? KPS * (lane & (NL - 1)) : lane & (KT - 1));
-    return key < k1 ? table[P.page_div.div((uint32_t)key)] : -1;
+    return table[min(P.page_div.div((uint32_t)key), (uint32_t)a.table_len - 1)];
   };
+  int pid = page_id(k0);
+  const SeqLens L = seq_lens(P, w.b);
+  const int rows = L.n * P.group;
+  if (r0 >= rows || w.split >= L.splits) return;
+  const int k1 = w.split == L.splits - 1 ? L.total : min(L.total, k0 + P.chunk);
   V8 kr[NL], vr[NL];
   uint64_t arrived = 0, present = 0;  // the keys that exist, of the tile being loaded and of the one at hand
   const int piece = tid & (PIECES - 1), ec = 8 * piece < D ? 8 * piece : 0, row = tid / PIECES;
   const uint32_t klane = (UNI ? row * P.k_slot : 0) + ec, vlane = (UNI ? row * P.v_slot : 0) + ec;
   auto issue = [&](int kt, int pid) {
     if constexpr (UNI) arrived = 0;
-    else arrived = __ballot((uint32_t)pid < (uint32_t)a.pages) & (KT == 64 ? ~0ull : (1ull << KT) - 1);
+    else arrived = __ballot((uint32_t)pid < (uint32_t)a.pages && kt + lane < k1) & (KT == 64 ? ~0ull : (1ull << KT) - 1);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int k = i * KPS + (UNI ? 0 : row);
@@ -553,7 +549,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
       int id;
       if constexpr (UNI) id = __builtin_amdgcn_readlane(pid, i);
       else id = __shfl(pid, k);
-      const bool ok = (uint32_t)id < (uint32_t)a.pages;
+      const bool ok = (uint32_t)id < (uint32_t)a.pages && (int)key < k1;
       const int own = ok ? -1 : 0;  // (all bits)
       const uint32_t page = id & own, off = (key - P.page_div.div(key) * a.page_size) & own;
       const uint64_t ko = (uint64_t)page * P.k_page + (uint64_t)off * P.k_slot;
@@ -561,12 +557,11 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
       const T* const vp = vbase + (P.one_offset ? ko : (uint64_t)page * P.v_page + (uint64_t)off * P.v_slot);
       kr[i] = piece_at(kp, klane);
       vr[i] = piece_at(vp, vlane);
-      if constexpr (UNI) arrived |= ok ? ((1ull << min(max(k1 - (int)key, 0), KPS)) - 1) << (i * KPS) : 0;
+      if constexpr (UNI) arrived |= ok ? ((1ull << min(k1 - (int)key, KPS)) - 1) << (i * KPS) : 0;
     }
   };
-  int pid = -1, next = -1;
+  int next = -1;
   if (k0 < k1) {
-    pid = page_id(k0);
     issue(k0, pid);
     next = page_id(k0 + KT);
   }
@@ -761,13 +756,18 @@ static TreePlan tree_plan(const fa_tree_attention_args* ap) {
   t.P.splits = 1;
   t.P.chunk = 1 << 30;
   if (a.seqs == 0 || a.nodes == 0) return t;
-  // keys are split until the launch has about four blocks a compute unit, in chunks of at least 256 keys
+  // The keys are split w ways so that rounds(w) (keys / w + 256), and 300 for the launch that joins them, is least: two blocks a
+  // compute unit are resident at once, and a block's beginning and end weigh about as much as 256 keys. (32 sequences of up to 2048 keys on 8 kv heads: 2 ways 50 us, 3:
+  // 60, 1: 57; 4 long ones with two row tiles: 8 ways 241 us, 16: 258.)
   const int64_t cap = (int64_t)a.table_len * a.page_size;
   const int64_t keys = std::max<int64_t>(1, std::min<int64_t>(cap, a.max_context > 0 ? (int64_t)a.max_context + a.nodes : cap));
-  const int64_t base = (int64_t)a.seqs * a.kv_heads * t.P.q_tiles;
-  const int64_t want = std::min<int64_t>(64, std::max<int64_t>(1, (4ll * cu_count() + base - 1) / base));
-  int64_t chunk = std::max<int64_t>(256, (keys + want - 1) / want);
-  chunk = (chunk + 127) / 128 * 128;
+  const int64_t base = (int64_t)a.seqs * a.kv_heads * t.P.q_tiles, slots = 2ll * cu_count();
+  int64_t ways = 1, least = INT64_MAX;
+  for (int64_t w = 1; w <= std::min<int64_t>(64, (keys + 127) / 128); ++w) {
+    const int64_t cost = (base * w + slots - 1) / slots * ((keys + w - 1) / w + 256) + (w > 1 ? 300 : 0);
+    if (cost < least) least = cost, ways = w;
+  }
+  const int64_t chunk = ((keys + ways - 1) / ways + 127) / 128 * 128;
   t.P.chunk = (int)chunk;
   t.P.splits = (int)((keys + chunk - 1) / chunk);
   t.P.q_tiles_div = FastDiv::of((uint32_t)std::max(1, t.P.q_tiles));
