@@ -9,16 +9,16 @@
 // whatever the order in which they are added: results do not depend on the launch shape or on atomics. The exponentials are
 // taken in 64 bits, because a sum over 150 000 tokens is compared with borders 7e-6 apart.
 //
-// A row is cut into chunks of 16 values a thread, one block each, so that a single row still uses many compute units:
+// A row is cut into chunks of 16 values a thread, one block each, so that a single row still uses many compute units; what
+// needs the whole row is done by one block of its own at the end. Four launches at most, two for most settings:
 //   k_scan    the chunk's maximum; with a small top_k also every thread's maximum.
-//   k_select  rows with a top_k up to KMAX: one block finishes the row. The k largest lie in the groups of 16 whose maximum is
-//             in the bins that hold k such maxima, so only those groups are read again (a few hundred values).
-//             rows with a top_p or a larger top_k: a histogram (count and mass by steps of 1/32 below the maximum); the block
-//             that arrives last finds the bins in which the cuts lie.
-//   k_draw    the other rows: each chunk's mass at the temperature, the values in the cuts' bins to a list; the block that
-//             arrives last sorts the list, fixes the cut, picks the chunk and the token in it.
-// Nothing waits for another block. A row whose cut's bins hold more than CAP values (thousands of equal logits) is finished
-// by one block that narrows the cut by key instead (general_row).
+//   k_hist    rows with a top_p or a top_k over KMAX: a histogram (count and mass by steps of 1/32 below the maximum); the block
+//             that arrives last finds the bins in which the cuts lie. Nothing waits for another block.
+//   k_mass    such rows, and rows with neither: each chunk's mass at the temperature; the values in the cuts' bins to a list.
+//   k_finish  one block a row. A top_k up to KMAX: the k largest lie in the groups of 16 whose maximum is in the bins that hold k
+//             such maxima, so only those groups are read again (a few hundred values). Else: the cut within the list by
+//             histograms of its entries, the chunk, the token in it. A row whose cut's bins hold more than CAP values
+//             (thousands of equal logits) is finished by narrowing the cut over the row itself (general_row).
 #include "api.h"
 #include "draft_ops.h"
 
@@ -29,14 +29,14 @@ namespace fa {
 constexpr int PER = 16;     // values a thread
 constexpr int BINS = 1024;  // of 1 / 32 below the maximum; the last takes everything 32 and more below
 constexpr int CAP = 4096;   // values that are sorted
-constexpr int ST = 1024;    // threads of k_select
-constexpr int KMAX = 1024;  // largest top_k that k_select finishes itself
+constexpr int ST = 1024;    // threads of k_hist and k_finish
+constexpr int KMAX = 1024;  // largest top_k that k_finish makes from the threads' maxima
 
 typedef unsigned long long u64;
 
 struct RowState {  // zeroed by k_scan
-  uint32_t arrived_select, arrived_draw, list_n, overflow;
-  int b_lo, b_hi, b_k, pad;  // bins of the cut: the listed ones are [b_lo, b_hi] and b_k
+  uint32_t arrived, list_n;
+  int b_lo, b_hi, b_k;       // bins of the cut: the listed ones are [b_lo, b_hi] and b_k
   u64 mass_lo, mass_k;       // mass before b_lo / before b_k
   u64 cnt_k;                 // values before b_k
   u64 total;                 // mass of the row
@@ -45,9 +45,9 @@ struct RowState {  // zeroed by k_scan
 struct SampleP {
   fa_sample_args a;
   double one;  // 2^S
-  int chunks;           // of PER values a thread of k_scan and k_draw
-  int sel_chunks;       // of k_select, whose blocks have ST threads whatever the others' have
-  FastDiv grid_div;     // blocks a row in this launch (1 where the first alone has work)
+  int chunks;           // of PER values a thread of k_scan and k_mass
+  int hist_chunks;      // of k_hist, whose blocks have ST threads whatever the others' have
+  FastDiv grid_div;     // blocks a row in this launch
   int grid_chunks;
   int want_max;  // the threads' maxima are wanted (a row may have a small top_k)
   float* cmax;   // [rows][chunks]
@@ -205,15 +205,14 @@ __device__ __forceinline__ X dev_add(X* p, X v) {
   return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <int BT>
+static_assert(ST == BINS, "a thread a bin");
 struct Shared {
   u64 mass[BINS];
   uint32_t cnt[BINS];
   u64 list[CAP];
-  u64 part[PER * BT / 64];
-  float wmax[BT / 64];
-  int widx[BT / 64], wcnt[BT / 64];
-  uint32_t wlo[BT / 64], whi[BT / 64];
+  u64 part[ST / 64], few[64], wmin[ST / 64], wmax[ST / 64];
+  int widx[ST / 64], wcnt[ST / 64];
+  uint32_t wlo[ST / 64], whi[ST / 64];
   int n, sel, flag, pick;
   u64 before_mass, mass_sel, total, chunk_before;
   uint32_t before_cnt;
@@ -221,18 +220,16 @@ struct Shared {
 };
 
 // true in the block that is the last of `n` to come here (block-uniform). Everything the block has handed over lies before
-template <int BT>
-__device__ __forceinline__ bool last_to_arrive(Shared<BT>& S, uint32_t* counter, int n) {
+__device__ __forceinline__ bool last_to_arrive(int& flag, uint32_t* counter, int n) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (threadIdx.x == 0) S.flag = dev_add(counter, 1u) == (uint32_t)n - 1;
+  if (threadIdx.x == 0) flag = dev_add(counter, 1u) == (uint32_t)n - 1;
   __syncthreads();
-  return S.flag != 0;
+  return flag != 0;
 }
 
 // the row's largest value and its lowest index, from the chunks' -> every thread
-template <int BT>
-__device__ __forceinline__ float row_top(Shared<BT>& S, const SampleP& P, int r, int& at) {
+__device__ __forceinline__ float row_top(const SampleP& P, int r, int& at) {
   const int lane = threadIdx.x & 63;
   float top = -INFINITY;
   at = 0x7FFFFFFF;
@@ -256,57 +253,49 @@ __device__ __forceinline__ float row_top(Shared<BT>& S, const SampleP& P, int r,
 }
 
 // first bin at which the running count reaches `need` or, by mass, the running mass reaches `target` -> S.sel, with what
-// lies before it in S.before_*; -1: none. Wave 0, 16 bins a lane. Ends with a barrier.
-template <int BT>
-__device__ __forceinline__ void find_bin(Shared<BT>& S, bool by_mass, uint32_t need, double target, uint32_t c0, u64 m0) {
-  if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
-    uint32_t c = 0, ci;
-    u64 m = 0, mi;
-#pragma unroll
-    for (int i = 0; i < BINS / 64; ++i) {
-      c += S.cnt[lane * (BINS / 64) + i];
-      m += S.mass[lane * (BINS / 64) + i];
-    }
-    ci = c;
-    mi = m;
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t cu = __shfl_up(ci, o);
-      const u64 mu = __shfl_up(mi, o);
-      if (lane >= o) {
-        ci += cu;
-        mi += mu;
-      }
-    }
-    const bool reached = by_mass ? (double)(m0 + mi) >= target : c0 + ci >= need;
-    const uint64_t who = __ballot(reached);
-    if (lane == 63) S.total = m0 + mi;
-    if (who == 0) {
-      if (lane == 0) S.sel = -1;
-    } else if (lane == first_lane(who)) {
-      uint32_t cb = c0 + ci - c;
-      u64 mb = m0 + mi - m;
-      int i = lane * (BINS / 64);
-      for (;; ++i) {
-        const uint32_t cn = cb + S.cnt[i];
-        const u64 mn = mb + S.mass[i];
-        if (by_mass ? (double)mn >= target : cn >= need) break;
-        cb = cn;
-        mb = mn;
-      }
-      S.sel = i;
-      S.before_cnt = cb;
-      S.before_mass = mb;
-    }
+// lies before it in S.before_*; -1: none. A thread a bin. Ends with a barrier.
+template <typename SH>
+__device__ __forceinline__ void find_bin(SH& S, bool by_mass, uint32_t need, double target, uint32_t c0, u64 m0) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t c = S.cnt[tid];
+  const u64 m = S.mass[tid];
+  uint32_t ci = c;
+  u64 mi = m;
+  if (by_mass) {
+    mi = wave_scan64(m, lane);
+  } else {
+    ci = (uint32_t)wave_scan64(c, lane);
+    mi = wave_scan64(m, lane);
   }
+  __syncthreads();  // (what an earlier call left has been read)
+  if (lane == 63) {
+    S.part[wave] = mi;
+    S.wcnt[wave] = (int)ci;
+  }
+  if (tid == 0) S.sel = -1;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) {
+    c0 += (uint32_t)S.wcnt[w];
+    m0 += S.part[w];
+  }
+  ci += c0;
+  mi += m0;
+  const bool reached = by_mass ? (double)mi >= target : ci >= need;
+  const bool before = by_mass ? (double)(mi - m) >= target : ci - c >= need;
+  if (reached && (!before || tid == 0)) {
+    S.sel = tid;
+    S.before_cnt = ci - c;
+    S.before_mass = mi - m;
+  }
+  if (tid == ST - 1) S.total = mi;
   __syncthreads();
 }
 
 // S.list[0 .. n) ascending; every entry is unique. A few hundred: each finds its own rank; more: bitonic
-template <int BT>
-__device__ __forceinline__ void sort_list(Shared<BT>& S, int n) {
+__device__ __forceinline__ void sort_list(Shared& S, int n) {
+  constexpr int BT = ST;
   const int tid = threadIdx.x;
-  if (n <= 256 && n <= BT) {
+  if (n <= 256) {
     u64 mine = 0;
     int rank = 0;
     if (tid < n) {
@@ -342,8 +331,7 @@ __device__ __forceinline__ uint32_t entry_key(u64 e) { return ~(uint32_t)(e >> 3
 
 // the first of the sorted list's values [i0, n) at which the mass, m0 lying before i0, reaches `target` -> its place, and the
 // mass up to and with it; -1: none. Every wave alike.
-template <int BT>
-__device__ __forceinline__ int list_reach(const Shared<BT>& S, int i0, int n, double target, u64 m0, float top, double one,
+__device__ __forceinline__ int list_reach(const Shared& S, int i0, int n, double target, u64 m0, float top, double one,
                                           u64& mass) {
   const int lane = threadIdx.x & 63;
   for (int i = i0; i < n; i += 64) {
@@ -371,9 +359,9 @@ __device__ __forceinline__ void put(const SampleP& P, int r, int token, u64 w, u
 
 // ------------------------------------------------------------------------------------------------------------ general row
 // One block finishes a row by narrowing the cut in the keys' space: no list that could overflow, many passes over the row.
-template <typename T, int BT>
-__device__ __forceinline__ void general_row(Shared<BT>& S, const SampleP& P, int r, float top) {
-  constexpr int NW = BT / 64;
+template <typename T>
+__device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, float top) {
+  constexpr int BT = ST, NW = BT / 64;
   const fa_sample_args& a = P.a;
   const RowSettings s = settings_of(a, r);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab;
@@ -631,9 +619,9 @@ __global__ __launch_bounds__(BT) void k_scan(SampleP P) {
   }
 }
 
-// a row with a small top_k, finished by one block. CT: threads of the blocks whose threads' maxima these are
+// a row with a small top_k. CT: threads of the blocks whose threads' maxima these are
 template <typename T, int CT>
-__device__ __forceinline__ void finish_small_k(Shared<ST>& S, const SampleP& P, int r, const RowSettings& s, float top) {
+__device__ __forceinline__ void finish_small_k(Shared& S, const SampleP& P, int r, const RowSettings& s, float top) {
   const int tid = threadIdx.x, lane = tid & 63;
   const RowView<T> v = row_view<T>(P.a, r);
   const float* const tm = P.tmax + (int64_t)r * P.chunks * CT;
@@ -644,20 +632,30 @@ __device__ __forceinline__ void finish_small_k(Shared<ST>& S, const SampleP& P, 
   S.mass[tid] = 0;
   if (tid == 0) S.n = S.pick = 0;
   __syncthreads();
-  for (int g = tid; g < groups; g += ST) {
+  // (the first rounds of maxima stay in registers: one wait for all of them)
+  constexpr int HOLD = 12;
+  float held[HOLD];
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i) held[i] = i * ST + tid < groups ? tm[i * ST + tid] : -INFINITY;
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i)
+    if (held[i] > -INFINITY) atomicAdd(&S.cnt[bin_of(held[i], top)], 1u);
+  for (int g = HOLD * ST + tid; g < groups; g += ST) {
     const float x = tm[g];
     if (x > -INFINITY) atomicAdd(&S.cnt[bin_of(x, top)], 1u);
   }
   __syncthreads();
   find_bin(S, false, (uint32_t)s.top_k, 0.0, 0, 0);
   const int b = S.sel < 0 ? BINS - 1 : S.sel;  // the k largest values lie in bins up to b
-  for (int g = tid; g < groups; g += ST) {
-    const float x = tm[g];
+  auto take = [&](int g, float x) {
     if (x > -INFINITY && bin_of(x, top) <= b) {
       const int j = atomicAdd(&S.pick, 1);
       if (j < PICK) pick[j] = (uint32_t)g;
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i) take(i * ST + tid, held[i]);
+  for (int g = HOLD * ST + tid; g < groups; g += ST) take(g, tm[g]);
   __syncthreads();
   const int ng = S.pick;
   if (ng <= PICK)
@@ -672,7 +670,7 @@ __device__ __forceinline__ void finish_small_k(Shared<ST>& S, const SampleP& P, 
     }
   __syncthreads();
   if (ng > PICK || S.n > CAP) {
-    general_row<T, ST>(S, P, r, top);
+    general_row<T>(S, P, r, top);
     return;
   }
   int n = S.n;
@@ -719,26 +717,22 @@ __device__ __forceinline__ void finish_small_k(Shared<ST>& S, const SampleP& P, 
   if (lane == 0) put(P, r, tok, wt, total);
 }
 
-static_assert(ST == BINS, "one bin a thread");
-template <typename T, int CT>
-__global__ __launch_bounds__(ST) void k_select(SampleP P) {
-  __shared__ Shared<ST> S;
+struct HistShared {  // what find_bin uses
+  u64 mass[BINS], part[ST / 64];
+  uint32_t cnt[BINS];
+  int wcnt[ST / 64], sel, flag;
+  u64 before_mass, total;
+  uint32_t before_cnt;
+};
+template <typename T>
+__global__ __launch_bounds__(ST, 8) void k_hist(SampleP P) {
+  __shared__ HistShared S;
   const int r = (int)P.grid_div.div(blockIdx.x), c = (int)blockIdx.x - r * P.grid_chunks;
   const RowSettings s = settings_of(P.a, r);
-  if (s.kind != HIST && !(s.kind == SMALL_K && c == 0)) return;
+  if (s.kind != HIST) return;
   int at;
-  const float top = row_top(S, P, r, at);
-  if (top == -INFINITY) {  // (HIST: k_draw answers)
-    if (s.kind == SMALL_K && threadIdx.x == 0) {
-      P.a.token_out[r] = -1;
-      if (P.a.prob_out) P.a.prob_out[r] = 0.f;
-    }
-    return;
-  }
-  if (s.kind == SMALL_K) {
-    finish_small_k<T, CT>(S, P, r, s, top);
-    return;
-  }
+  const float top = row_top(P, r, at);
+  if (top == -INFINITY) return;
   const int tid = threadIdx.x;
   S.cnt[tid] = 0;
   S.mass[tid] = 0;
@@ -749,7 +743,7 @@ __global__ __launch_bounds__(ST) void k_select(SampleP P) {
   for (int e = 0; e < PER; ++e) {
     if (x[e] == -INFINITY) continue;
     const int b = bin_of(x[e], top);
-    atomicAdd(&S.cnt[b], 1u);
+    if (s.has_k) atomicAdd(&S.cnt[b], 1u);
     if (s.has_p) atomicAdd(&S.mass[b], weight(rel_of(x[e], top), P.one));
   }
   __syncthreads();
@@ -758,7 +752,7 @@ __global__ __launch_bounds__(ST) void k_select(SampleP P) {
   if (S.cnt[tid]) dev_add(hc + tid, S.cnt[tid]);
   if (S.mass[tid]) dev_add(hm + tid, S.mass[tid]);
   RowState* const st = P.state + r;
-  if (!last_to_arrive(S, &st->arrived_select, P.sel_chunks)) return;
+  if (!last_to_arrive(S.flag, &st->arrived, P.hist_chunks)) return;
   S.cnt[tid] = dev_load(hc + tid);
   S.mass[tid] = dev_load(hm + tid);
   __syncthreads();
@@ -794,11 +788,6 @@ __global__ __launch_bounds__(ST) void k_select(SampleP P) {
     mass_lo = mass_k;
   }
   if (tid == 0) {
-    uint32_t n = 0;
-    if (b_lo >= 0)
-      for (int i = b_lo; i <= b_hi; ++i) n += S.cnt[i];
-    if (b_k > b_hi) n += S.cnt[b_k];
-    st->overflow = n > CAP;
     st->b_lo = b_lo < 0 ? BINS : b_lo;  // bins below b_lo are kept whole
     st->b_hi = b_hi;
     st->b_k = b_k;
@@ -810,182 +799,285 @@ __global__ __launch_bounds__(ST) void k_select(SampleP P) {
 }
 
 template <typename T, int BT>
-__global__ __launch_bounds__(BT, BT == 256 ? 4 : 1) void k_draw(SampleP P) {
-  __shared__ Shared<BT> S;
+__global__ __launch_bounds__(BT) void k_mass(SampleP P) {
+  __shared__ u64 part[BT / 64];
   const int r = (int)P.grid_div.div(blockIdx.x), c = (int)blockIdx.x - r * P.grid_chunks;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const RowSettings s = settings_of(P.a, r);
-  if (s.kind == SMALL_K || (s.kind == GREEDY && c != 0)) return;
-  int at;
-  const float top = row_top(S, P, r, at);
-  if (s.kind == GREEDY || top == -INFINITY) {
-    if (c == 0 && tid == 0) {
-      P.a.token_out[r] = top == -INFINITY ? -1 : at;
-      if (P.a.prob_out) P.a.prob_out[r] = top == -INFINITY ? 0.f : 1.f;
-    }
-    return;
-  }
-  RowState* const st = P.state + r;
-  const bool hist = s.kind == HIST;
-  if (hist && st->overflow) {
-    if (c == 0) general_row<T, BT>(S, P, r, top);
-    return;
-  }
-  const int b_lo = hist ? st->b_lo : BINS, b_hi = hist ? st->b_hi : -1, b_k = hist ? st->b_k : -1;
+  if (s.kind != HIST && s.kind != PLAIN) return;
   const RowView<T> v = row_view<T>(P.a, r);
   float x[PER];
   load_chunk<T, BT>(v, c * PER * BT, tid, x);
+  int at;
+  const float top = row_top(P, r, at);
+  if (top == -INFINITY) return;
+  RowState* const st = P.state + r;
+  const bool hist = s.kind == HIST;
+  const int b_lo = hist ? st->b_lo : BINS, b_hi = hist ? st->b_hi : -1, b_k = hist ? st->b_k : -1;
   u64 sum = 0;
+  uint32_t listed = 0;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    const bool some = x[e] > -INFINITY;
-    const int b = some ? bin_of(x[e], top) : BINS;
-    if (b < b_lo && some) {
+    if (x[e] == -INFINITY) continue;
+    const int b = bin_of(x[e], top);
+    if (b < b_lo) {
       const double rel = rel_of(x[e], top);
       if (!(rel < s.least)) sum += weight(rel * s.inv_t, P.one);
     }
-    const bool listed = some && ((b >= b_lo && b <= b_hi) || b == b_k);
-    const uint64_t who = __ballot(listed);
-    if (who) {
-      uint32_t j = 0;
-      if (lane == first_lane(who)) j = dev_add(&st->list_n, (uint32_t)__popcll(who));
-      j = __shfl(j, first_lane(who)) + __popcll(who & ((1ull << lane) - 1));
-      if (listed && j < CAP) dev_store(P.list + (int64_t)r * CAP + j, entry_of(x[e], index_at<T, BT>(v.vec, c * PER * BT, tid, e)));
+    if ((b >= b_lo && b <= b_hi) || b == b_k) listed |= 1u << e;
+  }
+  if (__any(listed != 0)) {  // a place in the row's list for the whole wave's, then for each lane's
+    const int own = __popc(listed);
+    int upto = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(upto, o);
+      if (lane >= o) upto += u;
     }
+    uint32_t j = 0;
+    if (lane == 63) j = dev_add(&st->list_n, (uint32_t)upto);
+    j = __shfl(j, 63) + upto - own;
+    u64* const list = P.list + (int64_t)r * CAP;
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (listed >> e & 1) {
+        if (j < CAP) list[j] = entry_of(x[e], index_at<T, BT>(v.vec, c * PER * BT, tid, e));
+        ++j;
+      }
   }
   sum = wave_sum64(sum);
-  if (lane == 0) S.part[wave] = sum;
+  if (lane == 0) part[wave] = sum;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < BT / 64; ++w) sum += S.part[w];
-    dev_store(P.cmass + (int64_t)r * P.chunks + c, sum);
+    for (int w = 1; w < BT / 64; ++w) sum += part[w];
+    P.cmass[(int64_t)r * P.chunks + c] = sum;
   }
-  if (!last_to_arrive(S, &st->arrived_draw, P.chunks)) return;
+}
 
-  // the cut
+// the cut among the listed entries (in S.list) that f accepts: the first, in their order, at which the count reaches `need` or
+// the mass `target`, c0 / m0 lying before them -> S.cut, S.mass_sel (mass up to it). Histograms of 1024 equal steps of the
+// entries' range, until 64 are left at most, which one wave sorts.
+template <typename F>
+__device__ __forceinline__ void refine_list(Shared& S, const SampleP& P, int n, F f, bool by_mass, uint32_t need, double target,
+                                            uint32_t c0, u64 m0, float top) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  u64 lo = 0, hi = ~0ull;
+  for (;;) {
+    u64 mn = ~0ull, mx = 0;
+    int own = 0;
+    for (int i = tid; i < n; i += ST) {
+      const u64 e = S.list[i];
+      if (e < lo || e > hi || !f(e)) continue;
+      mn = min(mn, e);
+      mx = max(mx, e);
+      ++own;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      mn = min(mn, (u64)__shfl_xor(mn, o));
+      mx = max(mx, (u64)__shfl_xor(mx, o));
+    }
+    own = wave_sum_i(own);
+    __syncthreads();
+    if (lane == 0) {
+      S.wmin[wave] = mn;
+      S.wmax[wave] = mx;
+      S.wcnt[wave] = own;
+    }
+    S.cnt[tid] = 0;
+    S.mass[tid] = 0;
+    if (tid == 0) S.n = 0;
+    __syncthreads();
+    own = 0;
+    for (int w = 0; w < ST / 64; ++w) {
+      mn = min(mn, S.wmin[w]);
+      mx = max(mx, S.wmax[w]);
+      own += S.wcnt[w];
+    }
+    lo = mn;
+    hi = mx;
+    if (own <= 64) break;
+    const int sh = max(0, 54 - __clzll((long long)(hi - lo)));  // (hi - lo) >> sh < 1024
+    for (int i = tid; i < n; i += ST) {
+      const u64 e = S.list[i];
+      if (e < lo || e > hi || !f(e)) continue;
+      const int q = (int)((e - lo) >> sh);
+      atomicAdd(&S.cnt[q], 1u);
+      if (by_mass) atomicAdd(&S.mass[q], weight(rel_of(key_value(entry_key(e)), top), P.one));
+    }
+    __syncthreads();
+    find_bin(S, by_mass, need, target, c0, m0);
+    const u64 q = (u64)S.sel;
+    c0 = S.before_cnt;
+    m0 = S.before_mass;
+    lo += q << sh;
+    hi = lo + min(hi - lo, (1ull << sh) - 1);
+  }
+  for (int i = tid; i < n; i += ST) {
+    const u64 e = S.list[i];
+    if (e >= lo && e <= hi && f(e)) S.few[atomicAdd(&S.n, 1)] = e;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const int m = S.n;
+    const u64 e = lane < m ? S.few[lane] : ~0ull;
+    int rank = 0;
+    for (int i = 0; i < m; ++i) rank += S.few[i] < e;
+    const u64 w = lane < m ? weight(rel_of(key_value(entry_key(e)), top), P.one) : 0;
+    u64 before = 0;  // mass of the smaller entries
+    for (int i = 0; i < m; ++i) {
+      const u64 wi = __shfl(w, i), ei = __shfl(e, i);
+      if (ei < e) before += wi;
+    }
+    const bool first = lane < m && (by_mass ? (double)(m0 + before + w) >= target && !((double)(m0 + before) >= target && rank > 0)
+                                            : c0 + rank + 1 == need);
+    if (first) {
+      S.cut = Cut{entry_key(e), (int)(uint32_t)e};
+      S.mass_sel = m0 + before + w;
+    }
+  }
+  __syncthreads();
+}
+
+// the rows that k_mass has prepared
+template <typename T, int CT>
+__device__ __forceinline__ void finish_masses(Shared& S, const SampleP& P, int r, const RowSettings& s, float top) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const RowState st = P.state[r];
+  const bool hist = s.kind == HIST;
+  const int n = hist ? (int)min(st.list_n, (uint32_t)(CAP + 1)) : 0;
+  if (n > CAP) {
+    general_row<T>(S, P, r, top);
+    return;
+  }
   Cut cut{0, 0x7FFFFFFF};
-  const int n = hist ? (int)dev_load(&st->list_n) : 0;
   u64* const cm = P.cmass + (int64_t)r * P.chunks;
   if (n > 0) {
-    for (int i = tid; i < n; i += BT) S.list[i] = dev_load(P.list + (int64_t)r * CAP + i);
+    for (int i = tid; i < n; i += ST) S.list[i] = P.list[(int64_t)r * CAP + i];
     __syncthreads();
-    sort_list(S, n);
-    int end = n;  // listed values within top_k
-    u64 total = st->total;
-    if (b_k >= 0) {
-      // the first listed value in bin b_k: everything in front of it lies in lower bins
-      int lo = 0, hi = n;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (bin_of(key_value(entry_key(S.list[mid])), top) < b_k) lo = mid + 1;
-        else hi = mid;
+    u64 total = st.total;
+    if (st.b_k >= 0) {
+      const int b_k = st.b_k;
+      refine_list(S, P, n, [&](u64 e) { return bin_of(key_value(entry_key(e)), top) == b_k; }, false, (uint32_t)s.top_k, 0.0,
+                  (uint32_t)st.cnt_k, 0, top);
+      cut = S.cut;
+      if (s.has_p) {  // the mass of the top_k
+        u64 m = 0;
+        for (int i = tid; i < n; i += ST) {
+          const u64 e = S.list[i];
+          const float x = key_value(entry_key(e));
+          if (bin_of(x, top) == b_k && within(entry_key(e), (int)(uint32_t)e, cut)) m += weight(rel_of(x, top), P.one);
+        }
+        m = wave_sum64(m);
+        if (lane == 0) S.part[wave] = m;
+        __syncthreads();
+        total = st.mass_k;
+        for (int w = 0; w < ST / 64; ++w) total += S.part[w];
+        __syncthreads();
       }
-      end = lo + (s.top_k - (int)st->cnt_k);
-      if (s.has_p) (void)list_reach(S, lo, end, INFINITY, st->mass_k, top, P.one, total);
     }
-    int last = end - 1;
     if (s.has_p) {
-      u64 mass;
-      last = list_reach(S, 0, end, (double)s.top_p * (double)total, st->mass_lo, top, P.one, mass);
+      // (between the listed bins and b_k lie values that are not listed; the target lies in the listed ones)
+      const int b_hi = st.b_hi;
+      const Cut lim = cut;
+      refine_list(S, P, n, [&](u64 e) {
+        return bin_of(key_value(entry_key(e)), top) <= b_hi && within(entry_key(e), (int)(uint32_t)e, lim);
+      }, true, 0, (double)s.top_p * (double)total, 0, st.mass_lo, top);
+      cut = S.cut;
     }
-    cut = Cut{entry_key(S.list[last]), (int)(uint32_t)S.list[last]};
-    // the kept ones' mass goes to their chunks (this block alone is left; its accesses go the same way as the others')
-    for (int i = tid; i <= last; i += BT) {
-      const double rel = rel_of(key_value(entry_key(S.list[i])), top);
-      if (!(rel < s.least))
-        dev_add(cm + (uint32_t)S.list[i] / (PER * BT), weight(rel * s.inv_t, P.one));
+    // the kept ones' mass goes to their chunks (no other block is at the row)
+    for (int i = tid; i < n; i += ST) {
+      const u64 e = S.list[i];
+      if (!within(entry_key(e), (int)(uint32_t)e, cut)) continue;
+      const double rel = rel_of(key_value(entry_key(e)), top);
+      if (!(rel < s.least)) dev_add(cm + (uint32_t)e / (PER * CT), weight(rel * s.inv_t, P.one));
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
-  // the chunk
-  if (wave == 0) {
-    u64 total = 0;
-    for (int i = lane; i < P.chunks; i += 64) total += dev_load(cm + i);
-    total = wave_sum64(total);
-    const double target = draw_target(P.a.u[r], total);
-    const bool past = !((double)total > target);
-    u64 before = 0, found = 0;
-    int pick = -1;
-    for (int i = 0; i < P.chunks; i += 64) {
-      const u64 w = i + lane < P.chunks ? dev_load(cm + i + lane) : 0;
-      const u64 mi = before + wave_scan64(w, lane);
-      const uint64_t who = __ballot(past ? w != 0 : (double)mi > target);
-      if (who) {
-        const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
-        pick = i + l;
-        found = __shfl(mi - w, l);
-        if (!past) break;
-      }
-      before = __shfl(mi, 63);
-    }
-    if (lane == 0) {
-      S.pick = pick;
-      S.chunk_before = found;
-      S.total = total;
-    }
-  }
-  __syncthreads();
-  // the token: sums of 64 W consecutive values in the order of the vocabulary, then the lane, then the value
-  const int pick = S.pick, base = pick * PER * BT;
-  const u64 total = S.total;
+  // the chunk: every wave alike
+  u64 total = 0;
+  for (int i = lane; i < P.chunks; i += 64) total += dev_load(cm + i);
+  total = wave_sum64(total);
   const double target = draw_target(P.a.u[r], total);
   const bool past = !((double)total > target);
-  load_chunk<T, BT>(v, base, tid, x);
-  u64 w[PER];
+  u64 before = 0, seen = 0;
+  int chunk = -1;
+  for (int i = 0; i < P.chunks; i += 64) {
+    const u64 w = i + lane < P.chunks ? dev_load(cm + i + lane) : 0;
+    const u64 mi = seen + wave_scan64(w, lane);
+    const uint64_t who = __ballot(past ? w != 0 : (double)mi > target);
+    seen = __shfl(mi, 63);
+    if (!who) continue;
+    const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
+    chunk = i + l;
+    before = __shfl(mi - w, l);
+    if (!past) break;
+  }
+  // the token: each thread PER CT / ST consecutive values of the chunk
+  constexpr int N = PER * CT / ST;
+  const RowView<T> v = row_view<T>(P.a, r);
+  const int i0 = chunk * PER * CT + tid * N;
+  u64 w[N], own = 0;
 #pragma unroll
-  for (int e = 0; e < PER; ++e) {
+  for (int e = 0; e < N; ++e) {
     w[e] = 0;
-    const int i = index_at<T, BT>(v.vec, base, tid, e);
-    if (x[e] > -INFINITY && within(order_key(x[e]), i, cut)) {
-      const double rel = rel_of(x[e], top);
+    const float x = i0 + e < v.V ? clean((float)v.p[i0 + e]) : -INFINITY;
+    if (x > -INFINITY && within(order_key(x), i0 + e, cut)) {
+      const double rel = rel_of(x, top);
       if (!(rel < s.least)) w[e] = weight(rel * s.inv_t, P.one);
     }
+    own += w[e];
   }
-  constexpr int NW = BT / 64;
-  const int W = v.vec ? kWide<T> : 1, runs = PER / W;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {  // a lane's sum of each run in w's last place of the run
-    if (e % W) w[e] += w[e - 1];
-    if (e % W == W - 1) {
-      const u64 t = wave_sum64(w[e]);
-      if (lane == 0) S.part[(e / W) * NW + wave] = t;
-    }
-  }
+  u64 mi = wave_scan64(own, lane);
+  if (lane == 63) S.part[wave] = mi;
   __syncthreads();
-  u64 before = S.chunk_before;
-  int cell = -1;
-  for (int i = 0; i < runs * NW; ++i) {
-    const u64 t = S.part[i];
-    if (past ? t != 0 : (double)(before + t) > target) {
-      cell = i;
-      if (!past) break;
-    }
-    if (!past) before += t;
+  u64 here = before;
+  for (int x = 0; x < wave; ++x) here += S.part[x];
+  mi += here;
+  // one thread's values hold the target: the first whose sum passes it, or past the end the last with any mass
+  bool mine;
+  if (past) {
+    const uint64_t who = __ballot(own != 0);
+    if (lane == 0) S.widx[wave] = who != 0;
+    __syncthreads();
+    int last = 0;
+    for (int x = 0; x < ST / 64; ++x)
+      if (S.widx[x]) last = x;
+    mine = wave == last && who && lane == 63 - __clzll((long long)who);
+  } else {
+    mine = (double)mi > target && !((double)(mi - own) > target);
   }
-  if (cell < 0 || wave != cell % NW) return;
-  const int run = cell / NW;
+  if (!mine) return;
+  u64 sum = mi - own, wt = 0;
+  int hit = -1;
 #pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    if (e / W != run || e % W != W - 1) continue;
-    const u64 mi = before + wave_scan64(w[e], lane);
-    const uint64_t who = __ballot(past ? w[e] != 0 : (double)mi > target);
-    const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
-    if (lane != l) continue;
-    // the value within the lane's run (w holds running sums)
-    const u64 b0 = mi - w[e];
-    int hit = -1;
-    u64 wt = 0;
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      if (q / W != run) continue;
-      const u64 prev = q % W ? w[q - 1] : 0, own = w[q] - prev;
-      if (own && (past || (hit < 0 && (double)(b0 + w[q]) > target))) {
-        hit = q;
-        wt = own;
-      }
+  for (int e = 0; e < N; ++e) {
+    sum += w[e];
+    if (w[e] && (past || (hit < 0 && (double)sum > target))) {
+      hit = e;
+      wt = w[e];
     }
-    put(P, r, index_at<T, BT>(v.vec, base, tid, hit), wt, total);
+  }
+  put(P, r, i0 + hit, wt, total);
+}
+
+template <typename T, int CT>
+__global__ __launch_bounds__(ST) void k_finish(SampleP P) {
+  __shared__ Shared S;
+  const int r = blockIdx.x;
+  const RowSettings s = settings_of(P.a, r);
+  int at;
+  const float top = row_top(P, r, at);
+  if (s.kind == GREEDY || top == -INFINITY) {
+    if (threadIdx.x == 0) {
+      P.a.token_out[r] = top == -INFINITY ? -1 : at;
+      if (P.a.prob_out) P.a.prob_out[r] = top == -INFINITY ? 0.f : 1.f;
+    }
+  } else if (s.kind == SMALL_K) {
+    finish_small_k<T, CT>(S, P, r, s, top);
+  } else {
+    finish_masses<T, CT>(S, P, r, s, top);
   }
 }
 
@@ -993,8 +1085,7 @@ __global__ __launch_bounds__(BT, BT == 256 ? 4 : 1) void k_draw(SampleP P) {
 struct SamplePlan {
   SampleP P;
   int bt;
-  bool select, draw;
-  int select_blocks, draw_blocks;  // a row
+  bool hist, mass;
   int64_t bytes;
 };
 
@@ -1013,17 +1104,15 @@ static SamplePlan sample_plan(const fa_sample_args* ap) {
   const int64_t small = (a.vocab + PER * 256 - 1) / (PER * 256);
   t.bt = a.rows * small <= 1024 ? 256 : 1024;
   t.P.chunks = (a.vocab + PER * t.bt - 1) / (PER * t.bt);
-  t.P.sel_chunks = (a.vocab + PER * ST - 1) / (PER * ST);
+  t.P.hist_chunks = (a.vocab + PER * ST - 1) / (PER * ST);
   FA_REQUIRE((int64_t)a.rows * t.P.chunks < (1ll << 31), "sample_tokens: more than 2^31 chunks");
   // which launches the rows can need (settings of each row live on the device: all)
   const bool each = a.temperatures || a.top_ps || a.min_ps || a.top_ks;
   const bool greedy = !(a.temperature > 0.f) || a.top_k == 1 || !(a.top_p > 0.f) || !(a.min_p <= 1.f);
   const bool has_k = a.top_k > 0 && a.top_k < a.vocab, small_k = has_k && a.top_k <= KMAX;
-  t.select = each || (!greedy && (has_k || a.top_p < 1.f));
-  t.draw = each || greedy || !small_k;
+  t.hist = each || (!greedy && !small_k && (has_k || a.top_p < 1.f));
+  t.mass = each || (!greedy && !small_k);
   t.P.want_max = each || (!greedy && small_k);
-  t.select_blocks = each || !small_k ? t.P.sel_chunks : 1;
-  t.draw_blocks = each || !greedy ? t.P.chunks : 1;
   const int64_t n = a.rows, nc = n * t.P.chunks;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1053,8 +1142,9 @@ static void sample_run(const SamplePlan& t, hipStream_t s) {
     launch(kernel, dim3((uint32_t)P.a.rows * (uint32_t)blocks), dim3(threads), 0, s, P);
   };
   go(k_scan<T, BT>, t.P.chunks, BT);
-  if (t.select) go(k_select<T, BT>, t.select_blocks, ST);
-  if (t.draw) go(k_draw<T, BT>, t.draw_blocks, BT);
+  if (t.hist) go(k_hist<T>, t.P.hist_chunks, ST);
+  if (t.mass) go(k_mass<T, BT>, t.P.chunks, BT);
+  go(k_finish<T, BT>, 1, ST);
 }
 
 static void sample_tokens(const fa_sample_args* ap, hipStream_t s) {
