@@ -71,11 +71,14 @@ inline void launch(void (*kernel)(P), dim3 grid, dim3 block, size_t lds, hipStre
   FA_HIP(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, args, lds, s));
 }
 
-// compute units of the current device (an attribute query: no allocation, no synchronisation, legal during capture)
+// compute units of the current device (an attribute query: no allocation, no synchronisation, legal during capture). It shapes
+// a launch only: without a device the MI355X's number, and the launch reports what is wrong
 inline int cu_count() {
   int dev = 0, n = 0;
-  FA_HIP(hipGetDevice(&dev));
-  FA_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) {
+    (void)hipGetLastError();
+    return 256;
+  }
   return n;
 }
 

@@ -5,9 +5,9 @@
 // cut (key of the last logit kept, last id kept among its equals), nothing is sorted but the few values near a cut, and the
 // draw runs through the vocabulary in its own order.
 //
-// Weights exp(x - max) are rounded to integers of 2^-S of the largest (S = 62 - ceil(log2 vocab)), so that sums are exact
-// whatever the order in which they are added: results do not depend on the launch shape or on atomics. The exponentials are
-// taken in 64 bits, because a sum over 150 000 tokens is compared with borders 7e-6 apart.
+// Weights exp(x - max) are rounded to integers of 2^-S of the largest (S = 62 - ceil(log2 vocab), at most 50), so that sums
+// are exact whatever the order in which they are added: results do not depend on the launch shape or on atomics. The
+// exponentials are taken in 64 bits, because a sum over 150 000 tokens is compared with borders 7e-6 apart.
 //
 // A row is cut into chunks of 16 values a thread, one block each, so that a single row still uses many compute units; what
 // needs the whole row is done by one block of its own at the end. Four launches at most, two for most settings:
@@ -44,9 +44,9 @@ struct RowState {  // zeroed by k_scan
 
 struct SampleP {
   fa_sample_args a;
-  double one;  // 2^S
+  int S;  // a weight of 1 is 2^S
   int chunks;           // of PER values a thread of k_scan and k_mass
-  int hist_chunks;      // of k_hist, whose blocks have ST threads whatever the others' have
+  int hist_chunks;      // k_hist's blocks a row
   FastDiv grid_div;     // blocks a row in this launch
   int grid_chunks;
   int want_max;  // the threads' maxima are wanted (a row may have a small top_k)
@@ -98,13 +98,16 @@ __device__ __forceinline__ int bin_of(float x, float top) {
   return x == top ? 0 : (int)fminf((top - x) * 32.f, (float)(BINS - 1));
 }
 __device__ __forceinline__ double rel_of(float x, float top) { return x == top ? 0.0 : (double)x - (double)top; }
-// exp(x) 2^S, rounded, for x <= 0: x = n ln 2 + 4 r with |r| <= ln 2 / 8, the Taylor polynomial of degree 9 in r
-// (remainder r^10 / 10! < 7e-18 of 1), squared twice: relative error below 4e-15 before the rounding to an integer
-__device__ __forceinline__ u64 weight(double x, double one) {
-  if (!(x > -60.0)) return 0;  // 2^62 exp(-60) < 1/2 (NaN: -inf times 1 / inf)
-  const double n = rint(x * 1.4426950408889634);
-  double r = fma(n, -0x1.62e42fefa39efp-1, x);
-  r = fma(n, -0x1.abc9e3b39803fp-56, r) * 0.25;
+// exp(x) 2^S, rounded to an integer, for x <= 0 and S <= 50: x = n ln 2 + 4 r with |r| <= ln 2 / 8, the Taylor polynomial of
+// degree 9 in r (remainder r^10 / 10! < 7e-18 of 1), squared twice: relative error below 4e-15 before the rounding. Adding
+// 1.5 2^52 leaves n, adding 2^52 the result, in the low bits of a sum: no conversions
+__device__ __forceinline__ u64 weight(double x, int S) {
+  if (!(x > -60.0)) return 0;  // 2^50 exp(-60) < 1/2 (NaN: -inf times 1 / inf)
+  const double t = fma(x, 1.4426950408889634, 0x1.8p52);
+  const int n = (int)(uint32_t)__double_as_longlong(t);
+  const double nf = t - 0x1.8p52;
+  double r = fma(nf, -0x1.62e42fefa39efp-1, x);
+  r = fma(nf, -0x1.abc9e3b39803fp-56, r) * 0.25;
   double p = 1.0 / 362880.0;
   p = fma(p, r, 1.0 / 40320.0);
   p = fma(p, r, 1.0 / 5040.0);
@@ -117,7 +120,8 @@ __device__ __forceinline__ u64 weight(double x, double one) {
   p = fma(p, r, 1.0);
   p *= p;
   p *= p;
-  return (u64)(ldexp(p, (int)n) * one + 0.5);
+  const double scale = __longlong_as_double((long long)(n + S + 1023) << 52);  // 2^(n + S), n + S >= -49
+  return (u64)__double_as_longlong(fma(p, scale, 0x1p52)) - 0x4330000000000000ull;
 }
 
 struct Cut {  // the last value kept
@@ -150,12 +154,12 @@ __device__ __forceinline__ int index_at(bool vec, int base, int t, int e) {
   constexpr int W = kWide<T>;
   return vec ? base + ((e / W) * BT + t) * W + e % W : base + e * BT + t;
 }
-template <typename T, int BT>
-__device__ __forceinline__ void load_chunk(const RowView<T>& v, int base, int t, float (&x)[PER]) {
+template <typename T, int BT, int N>
+__device__ __forceinline__ void load_chunk(const RowView<T>& v, int base, int t, float (&x)[N]) {
   constexpr int W = kWide<T>;
   if (v.vec) {
 #pragma unroll
-    for (int j = 0; j < PER / W; ++j) {
+    for (int j = 0; j < N / W; ++j) {
       const int i = base + (j * BT + t) * W;
       T y[W];
       if (i + W <= v.V) {
@@ -169,26 +173,34 @@ __device__ __forceinline__ void load_chunk(const RowView<T>& v, int base, int t,
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
+    for (int e = 0; e < N; ++e) {
       const int i = base + e * BT + t;
       x[e] = i < v.V ? clean((float)v.p[i]) : -INFINITY;
     }
   }
 }
 
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+// 64-bit sums over a wave by data-parallel moves: within rows of 16 lanes by 1, 2, 4, 8, then a row's last lane to the rows
+// behind it (a shuffle through LDS takes ten times as long). Lanes that a move does not reach add 0
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved64(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+  return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 wave_scan64(u64 v) {  // inclusive; every lane active
+  v += moved64<0x111, 0xF>(v);
+  v += moved64<0x112, 0xF>(v);
+  v += moved64<0x114, 0xF>(v);
+  v += moved64<0x118, 0xF>(v);
+  v += moved64<0x142, 0xA>(v);
+  v += moved64<0x143, 0xC>(v);
   return v;
 }
-__device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
-  return v;
+__device__ __forceinline__ u64 lane64(u64 v, int l) {  // a lane's value, l the same in all
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
 }
+__device__ __forceinline__ u64 wave_sum64(u64 v) { return lane64(wave_scan64(v), 63); }
 __device__ __forceinline__ int first_lane(uint64_t m) { return __ffsll((unsigned long long)m) - 1; }
 
 // values that blocks of one launch hand to each other pass the per-XCD caches: relaxed device-scope accesses
@@ -210,11 +222,11 @@ struct Shared {
   u64 mass[BINS];
   uint32_t cnt[BINS];
   u64 list[CAP];
-  u64 part[ST / 64], few[64], wmin[ST / 64], wmax[ST / 64];
+  u64 part[ST / 64], few[64], lo, hi;
   int widx[ST / 64], wcnt[ST / 64];
   uint32_t wlo[ST / 64], whi[ST / 64];
-  int n, sel, flag, pick;
-  u64 before_mass, mass_sel, total, chunk_before;
+  int n, sel, pick;
+  u64 before_mass, mass_sel, total;
   uint32_t before_cnt;
   Cut cut;
 };
@@ -260,13 +272,8 @@ __device__ __forceinline__ void find_bin(SH& S, bool by_mass, uint32_t need, dou
   const uint32_t c = S.cnt[tid];
   const u64 m = S.mass[tid];
   uint32_t ci = c;
-  u64 mi = m;
-  if (by_mass) {
-    mi = wave_scan64(m, lane);
-  } else {
-    ci = (uint32_t)wave_scan64(c, lane);
-    mi = wave_scan64(m, lane);
-  }
+  u64 mi = wave_scan64(m);
+  if (!by_mass) ci = (uint32_t)wave_scan64(c);
   __syncthreads();  // (what an earlier call left has been read)
   if (lane == 63) {
     S.part[wave] = mi;
@@ -274,9 +281,10 @@ __device__ __forceinline__ void find_bin(SH& S, bool by_mass, uint32_t need, dou
   }
   if (tid == 0) S.sel = -1;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    c0 += (uint32_t)S.wcnt[w];
-    m0 += S.part[w];
+#pragma unroll
+  for (int w = 0; w < ST / 64; ++w) {
+    c0 += w < wave ? (uint32_t)S.wcnt[w] : 0;
+    m0 += w < wave ? S.part[w] : 0;
   }
   ci += c0;
   mi += m0;
@@ -296,11 +304,16 @@ __device__ __forceinline__ void sort_list(Shared& S, int n) {
   constexpr int BT = ST;
   const int tid = threadIdx.x;
   if (n <= 256) {
+    const int m = (n + 7) / 8 * 8;  // eight reads at once
+    if (tid >= n && tid < m) S.list[tid] = ~0ull;
+    __syncthreads();
     u64 mine = 0;
     int rank = 0;
     if (tid < n) {
       mine = S.list[tid];
-      for (int i = 0; i < n; ++i) rank += S.list[i] < mine;
+      for (int i = 0; i < m; i += 8)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) rank += S.list[i + q] < mine;
     }
     __syncthreads();
     if (tid < n) S.list[rank] = mine;
@@ -331,19 +344,19 @@ __device__ __forceinline__ uint32_t entry_key(u64 e) { return ~(uint32_t)(e >> 3
 
 // the first of the sorted list's values [i0, n) at which the mass, m0 lying before i0, reaches `target` -> its place, and the
 // mass up to and with it; -1: none. Every wave alike.
-__device__ __forceinline__ int list_reach(const Shared& S, int i0, int n, double target, u64 m0, float top, double one,
+__device__ __forceinline__ int list_reach(const Shared& S, int i0, int n, double target, u64 m0, float top, int S_,
                                           u64& mass) {
   const int lane = threadIdx.x & 63;
   for (int i = i0; i < n; i += 64) {
-    const u64 w = i + lane < n ? weight(rel_of(key_value(entry_key(S.list[i + lane])), top), one) : 0;
-    const u64 mi = m0 + wave_scan64(w, lane);
+    const u64 w = i + lane < n ? weight(rel_of(key_value(entry_key(S.list[i + lane])), top), S_) : 0;
+    const u64 mi = m0 + wave_scan64(w);
     const uint64_t who = __ballot(i + lane < n && (double)mi >= target);
     if (who) {
       const int l = first_lane(who);
-      mass = __shfl(mi, l);
+      mass = lane64(mi, l);
       return i + l;
     }
-    m0 = __shfl(mi, 63);
+    m0 = lane64(mi, 63);
   }
   mass = m0;
   return -1;
@@ -414,7 +427,7 @@ __device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, 
       hi = mx;
       if (n <= CAP) break;
       if (lo == hi) {  // equal values: so many of them, in the order of their ids
-        const u64 w = weight(rel_of(key_value(lo), top), P.one);
+        const u64 w = weight(rel_of(key_value(lo), top), P.S);
         uint32_t c = need - c0;
         if (by_mass) {
           const double f = ceil((target - (double)m0) / (double)w);
@@ -458,7 +471,7 @@ __device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, 
       each([&](float x, uint32_t k, int) {
         const int q = (int)((hi - k) >> sh);
         atomicAdd(&S.cnt[q], 1u);
-        if (s.has_p) atomicAdd(&S.mass[q], weight(rel_of(x, top), P.one));
+        if (s.has_p) atomicAdd(&S.mass[q], weight(rel_of(x, top), P.S));
       });
       __syncthreads();
       find_bin(S, by_mass, need, target, c0, m0);
@@ -476,8 +489,8 @@ __device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, 
     sort_list(S, n);
     u64 mass = 0;
     int at = (int)(need - c0) - 1;
-    if (by_mass) at = list_reach(S, 0, n, target, m0, top, P.one, mass);
-    else if (s.has_p) (void)list_reach(S, 0, at + 1, INFINITY, m0, top, P.one, mass);
+    if (by_mass) at = list_reach(S, 0, n, target, m0, top, P.S, mass);
+    else if (s.has_p) (void)list_reach(S, 0, at + 1, INFINITY, m0, top, P.S, mass);
     if (tid == 0) {
       S.cut = Cut{entry_key(S.list[at]), (int)(uint32_t)S.list[at]};
       S.mass_sel = mass;
@@ -498,7 +511,7 @@ __device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, 
         if (x == -INFINITY || !within(order_key(x), i, cut)) continue;
         const int b = bin_of(x, top);
         atomicAdd(&S.cnt[b], 1u);
-        if (s.has_p) atomicAdd(&S.mass[b], weight(rel_of(x, top), P.one));
+        if (s.has_p) atomicAdd(&S.mass[b], weight(rel_of(x, top), P.S));
       }
       __syncthreads();
     };
@@ -531,7 +544,7 @@ __device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, 
     const float x = logit(i);
     if (x == -INFINITY || !within(order_key(x), i, cut)) return 0;
     const double rel = rel_of(x, top);
-    return rel < s.least ? 0 : weight(rel * s.inv_t, P.one);
+    return rel < s.least ? 0 : weight(rel * s.inv_t, P.S);
   };
   const int seg = ((V + NW - 1) / NW + 63) / 64 * 64, i0 = min(V, wave * seg), i1 = min(V, i0 + seg);
   u64 sum = 0;
@@ -555,13 +568,13 @@ __device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, 
     u64 wt = 0;
     for (int i = i0; i < i1; i += 64) {
       const u64 w = i + lane < i1 ? mass_at(i + lane) : 0;
-      const u64 mi = before + wave_scan64(w, lane);
+      const u64 mi = before + wave_scan64(w);
       const uint64_t who = __ballot(past ? w != 0 : (double)mi > target);
-      before = __shfl(mi, 63);
+      before = lane64(mi, 63);
       if (!who) continue;
       const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
       tok = i + l;
-      wt = __shfl(w, l);
+      wt = lane64(w, l);
       if (!past) break;
     }
     if (lane == 0) put(P, r, tok, wt, total);
@@ -577,7 +590,7 @@ __global__ __launch_bounds__(BT) void k_scan(SampleP P) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, base = c * PER * BT;
   const RowView<T> v = row_view<T>(P.a, r);
   float x[PER];
-  load_chunk<T, BT>(v, base, tid, x);
+  load_chunk<T, BT, PER>(v, base, tid, x);
   float top = x[0];
 #pragma unroll
   for (int e = 1; e < PER; ++e) top = fmaxf(top, x[e]);
@@ -678,15 +691,15 @@ __device__ __forceinline__ void finish_small_k(Shared& S, const SampleP& P, int 
   n = min(n, s.top_k);
   if (s.has_p) {
     u64 total = 0, mass;
-    (void)list_reach(S, 0, n, INFINITY, 0, top, P.one, total);
-    n = 1 + list_reach(S, 0, n, (double)s.top_p * (double)total, 0, top, P.one, mass);
+    (void)list_reach(S, 0, n, INFINITY, 0, top, P.S, total);
+    n = 1 + list_reach(S, 0, n, (double)s.top_p * (double)total, 0, top, P.S, mass);
   }
   // weights at the temperature (the values that min_p drops are the last ones: no weight), then the order of the ids
   u64 w = 0, e = 0;
   if (tid < n) {
     e = S.list[tid];
     const double rel = rel_of(key_value(entry_key(e)), top);
-    w = rel < s.least ? 0 : weight(rel * s.inv_t, P.one);
+    w = rel < s.least ? 0 : weight(rel * s.inv_t, P.S);
   }
   __syncthreads();
   if (tid < n) {
@@ -705,13 +718,13 @@ __device__ __forceinline__ void finish_small_k(Shared& S, const SampleP& P, int 
   int tok = -1;
   for (int i = 0; i < n; i += 64) {
     const u64 q = i + lane < n ? S.list[i + lane] : 0;
-    const u64 m = i + lane < n ? S.mass[(uint32_t)q] : 0, mi = before + wave_scan64(m, lane);
+    const u64 m = i + lane < n ? S.mass[(uint32_t)q] : 0, mi = before + wave_scan64(m);
     const uint64_t who = __ballot(past ? m != 0 : (double)mi > target);
-    before = __shfl(mi, 63);
+    before = lane64(mi, 63);
     if (!who) continue;
     const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
-    tok = (int)(__shfl(q, l) >> 32);
-    wt = __shfl(m, l);
+    tok = (int)(lane64(q, l) >> 32);
+    wt = lane64(m, l);
     if (!past) break;
   }
   if (lane == 0) put(P, r, tok, wt, total);
@@ -736,15 +749,16 @@ __global__ __launch_bounds__(ST, 8) void k_hist(SampleP P) {
   const int tid = threadIdx.x;
   S.cnt[tid] = 0;
   S.mass[tid] = 0;
-  float x[PER];
-  load_chunk<T, ST>(row_view<T>(P.a, r), c * PER * ST, tid, x);
   __syncthreads();
+  const RowView<T> v = row_view<T>(P.a, r);
+  float x[PER];
+  load_chunk<T, ST, PER>(v, c * PER * ST, tid, x);
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     if (x[e] == -INFINITY) continue;
     const int b = bin_of(x[e], top);
     if (s.has_k) atomicAdd(&S.cnt[b], 1u);
-    if (s.has_p) atomicAdd(&S.mass[b], weight(rel_of(x[e], top), P.one));
+    if (s.has_p) atomicAdd(&S.mass[b], weight(rel_of(x[e], top), P.S));
   }
   __syncthreads();
   u64* const hm = P.hist_mass + (int64_t)r * BINS;
@@ -807,7 +821,7 @@ __global__ __launch_bounds__(BT) void k_mass(SampleP P) {
   if (s.kind != HIST && s.kind != PLAIN) return;
   const RowView<T> v = row_view<T>(P.a, r);
   float x[PER];
-  load_chunk<T, BT>(v, c * PER * BT, tid, x);
+  load_chunk<T, BT, PER>(v, c * PER * BT, tid, x);
   int at;
   const float top = row_top(P, r, at);
   if (top == -INFINITY) return;
@@ -822,7 +836,7 @@ __global__ __launch_bounds__(BT) void k_mass(SampleP P) {
     const int b = bin_of(x[e], top);
     if (b < b_lo) {
       const double rel = rel_of(x[e], top);
-      if (!(rel < s.least)) sum += weight(rel * s.inv_t, P.one);
+      if (!(rel < s.least)) sum += weight(rel * s.inv_t, P.S);
     }
     if ((b >= b_lo && b <= b_hi) || b == b_k) listed |= 1u << e;
   }
@@ -863,6 +877,15 @@ __device__ __forceinline__ void refine_list(Shared& S, const SampleP& P, int n, 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   u64 lo = 0, hi = ~0ull;
   for (;;) {
+    __syncthreads();
+    S.cnt[tid] = 0;
+    S.mass[tid] = 0;
+    if (tid == 0) {
+      S.n = 0;
+      S.lo = ~0ull;
+      S.hi = 0;
+    }
+    __syncthreads();
     u64 mn = ~0ull, mx = 0;
     int own = 0;
     for (int i = tid; i < n; i += ST) {
@@ -872,30 +895,15 @@ __device__ __forceinline__ void refine_list(Shared& S, const SampleP& P, int n, 
       mx = max(mx, e);
       ++own;
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      mn = min(mn, (u64)__shfl_xor(mn, o));
-      mx = max(mx, (u64)__shfl_xor(mx, o));
+    if (own) {  // (of a few values a thread, by LDS atomics)
+      atomicMin(&S.lo, mn);
+      atomicMax(&S.hi, mx);
+      atomicAdd(&S.n, own);
     }
-    own = wave_sum_i(own);
     __syncthreads();
-    if (lane == 0) {
-      S.wmin[wave] = mn;
-      S.wmax[wave] = mx;
-      S.wcnt[wave] = own;
-    }
-    S.cnt[tid] = 0;
-    S.mass[tid] = 0;
-    if (tid == 0) S.n = 0;
-    __syncthreads();
-    own = 0;
-    for (int w = 0; w < ST / 64; ++w) {
-      mn = min(mn, S.wmin[w]);
-      mx = max(mx, S.wmax[w]);
-      own += S.wcnt[w];
-    }
-    lo = mn;
-    hi = mx;
+    lo = S.lo;
+    hi = S.hi;
+    own = S.n;
     if (own <= 64) break;
     const int sh = max(0, 54 - __clzll((long long)(hi - lo)));  // (hi - lo) >> sh < 1024
     for (int i = tid; i < n; i += ST) {
@@ -903,7 +911,7 @@ __device__ __forceinline__ void refine_list(Shared& S, const SampleP& P, int n, 
       if (e < lo || e > hi || !f(e)) continue;
       const int q = (int)((e - lo) >> sh);
       atomicAdd(&S.cnt[q], 1u);
-      if (by_mass) atomicAdd(&S.mass[q], weight(rel_of(key_value(entry_key(e)), top), P.one));
+      if (by_mass) atomicAdd(&S.mass[q], weight(rel_of(key_value(entry_key(e)), top), P.S));
     }
     __syncthreads();
     find_bin(S, by_mass, need, target, c0, m0);
@@ -913,20 +921,22 @@ __device__ __forceinline__ void refine_list(Shared& S, const SampleP& P, int n, 
     lo += q << sh;
     hi = lo + min(hi - lo, (1ull << sh) - 1);
   }
+  if (tid == 0) S.sel = 0;
+  __syncthreads();
   for (int i = tid; i < n; i += ST) {
     const u64 e = S.list[i];
-    if (e >= lo && e <= hi && f(e)) S.few[atomicAdd(&S.n, 1)] = e;
+    if (e >= lo && e <= hi && f(e)) S.few[atomicAdd(&S.sel, 1)] = e;
   }
   __syncthreads();
   if (wave == 0) {
-    const int m = S.n;
+    const int m = S.sel;
     const u64 e = lane < m ? S.few[lane] : ~0ull;
     int rank = 0;
     for (int i = 0; i < m; ++i) rank += S.few[i] < e;
-    const u64 w = lane < m ? weight(rel_of(key_value(entry_key(e)), top), P.one) : 0;
+    const u64 w = lane < m ? weight(rel_of(key_value(entry_key(e)), top), P.S) : 0;
     u64 before = 0;  // mass of the smaller entries
     for (int i = 0; i < m; ++i) {
-      const u64 wi = __shfl(w, i), ei = __shfl(e, i);
+      const u64 wi = lane64(w, i), ei = lane64(e, i);
       if (ei < e) before += wi;
     }
     const bool first = lane < m && (by_mass ? (double)(m0 + before + w) >= target && !((double)(m0 + before) >= target && rank > 0)
@@ -943,6 +953,11 @@ __device__ __forceinline__ void refine_list(Shared& S, const SampleP& P, int n, 
 template <typename T, int CT>
 __device__ __forceinline__ void finish_masses(Shared& S, const SampleP& P, int r, const RowSettings& s, float top) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // (everything that k_mass has left, in one wait: list entries behind list_n are read and not used)
+  u64 entry[CAP / ST];
+#pragma unroll
+  for (int q = 0; q < CAP / ST; ++q) entry[q] = P.list[(int64_t)r * CAP + q * ST + tid];
+  const u64 own_chunk = tid < P.chunks ? P.cmass[(int64_t)r * P.chunks + tid] : 0;
   const RowState st = P.state[r];
   const bool hist = s.kind == HIST;
   const int n = hist ? (int)min(st.list_n, (uint32_t)(CAP + 1)) : 0;
@@ -951,11 +966,12 @@ __device__ __forceinline__ void finish_masses(Shared& S, const SampleP& P, int r
     return;
   }
   Cut cut{0, 0x7FFFFFFF};
-  u64* const cm = P.cmass + (int64_t)r * P.chunks;
   if (n > 0) {
-    for (int i = tid; i < n; i += ST) S.list[i] = P.list[(int64_t)r * CAP + i];
+#pragma unroll
+    for (int q = 0; q < CAP / ST; ++q)
+      if (q * ST + tid < n) S.list[q * ST + tid] = entry[q];
     __syncthreads();
-    u64 total = st.total;
+    u64 total = st.total;  // of the top_k
     if (st.b_k >= 0) {
       const int b_k = st.b_k;
       refine_list(S, P, n, [&](u64 e) { return bin_of(key_value(entry_key(e)), top) == b_k; }, false, (uint32_t)s.top_k, 0.0,
@@ -966,7 +982,7 @@ __device__ __forceinline__ void finish_masses(Shared& S, const SampleP& P, int r
         for (int i = tid; i < n; i += ST) {
           const u64 e = S.list[i];
           const float x = key_value(entry_key(e));
-          if (bin_of(x, top) == b_k && within(entry_key(e), (int)(uint32_t)e, cut)) m += weight(rel_of(x, top), P.one);
+          if (bin_of(x, top) == b_k && within(entry_key(e), (int)(uint32_t)e, cut)) m += weight(rel_of(x, top), P.S);
         }
         m = wave_sum64(m);
         if (lane == 0) S.part[wave] = m;
@@ -985,35 +1001,40 @@ __device__ __forceinline__ void finish_masses(Shared& S, const SampleP& P, int r
       }, true, 0, (double)s.top_p * (double)total, 0, st.mass_lo, top);
       cut = S.cut;
     }
-    // the kept ones' mass goes to their chunks (no other block is at the row)
-    for (int i = tid; i < n; i += ST) {
-      const u64 e = S.list[i];
-      if (!within(entry_key(e), (int)(uint32_t)e, cut)) continue;
-      const double rel = rel_of(key_value(entry_key(e)), top);
-      if (!(rel < s.least)) dev_add(cm + (uint32_t)e / (PER * CT), weight(rel * s.inv_t, P.one));
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
   }
-  // the chunk: every wave alike
-  u64 total = 0;
-  for (int i = lane; i < P.chunks; i += 64) total += dev_load(cm + i);
-  total = wave_sum64(total);
+  // the chunks' masses, with the kept listed values' (a thread a chunk)
+  __syncthreads();
+  S.mass[tid] = own_chunk;
+  __syncthreads();
+  for (int i = tid; i < n; i += ST) {
+    const u64 e = S.list[i];
+    if (!within(entry_key(e), (int)(uint32_t)e, cut)) continue;
+    const double rel = rel_of(key_value(entry_key(e)), top);
+    if (!(rel < s.least)) atomicAdd(&S.mass[(uint32_t)e / (PER * CT)], weight(rel * s.inv_t, P.S));
+  }
+  __syncthreads();
+  // the chunk: the first whose sum passes the target, or past the end the last with any mass
+  const u64 cw = S.mass[tid], cs = wave_scan64(cw);
+  if (lane == 63) S.part[wave] = cs;
+  if (tid == 0) S.pick = -1;
+  __syncthreads();
+  u64 ahead = 0, total = 0;
+#pragma unroll
+  for (int x = 0; x < ST / 64; ++x) {
+    ahead += x < wave ? S.part[x] : 0;
+    total += S.part[x];
+  }
   const double target = draw_target(P.a.u[r], total);
   const bool past = !((double)total > target);
-  u64 before = 0, seen = 0;
-  int chunk = -1;
-  for (int i = 0; i < P.chunks; i += 64) {
-    const u64 w = i + lane < P.chunks ? dev_load(cm + i + lane) : 0;
-    const u64 mi = seen + wave_scan64(w, lane);
-    const uint64_t who = __ballot(past ? w != 0 : (double)mi > target);
-    seen = __shfl(mi, 63);
-    if (!who) continue;
-    const int l = past ? 63 - __clzll((long long)who) : first_lane(who);
-    chunk = i + l;
-    before = __shfl(mi - w, l);
-    if (!past) break;
+  if (past) {
+    if (cw) atomicMax(&S.pick, tid);
+  } else if ((double)(ahead + cs) > target && !((double)(ahead + cs - cw) > target)) {
+    S.pick = tid;
+    S.before_mass = ahead + cs - cw;
   }
+  __syncthreads();
+  const int chunk = S.pick;
+  const u64 before = S.before_mass;  // (past the end: not looked at)
   // the token: each thread PER CT / ST consecutive values of the chunk
   constexpr int N = PER * CT / ST;
   const RowView<T> v = row_view<T>(P.a, r);
@@ -1025,15 +1046,16 @@ __device__ __forceinline__ void finish_masses(Shared& S, const SampleP& P, int r
     const float x = i0 + e < v.V ? clean((float)v.p[i0 + e]) : -INFINITY;
     if (x > -INFINITY && within(order_key(x), i0 + e, cut)) {
       const double rel = rel_of(x, top);
-      if (!(rel < s.least)) w[e] = weight(rel * s.inv_t, P.one);
+      if (!(rel < s.least)) w[e] = weight(rel * s.inv_t, P.S);
     }
     own += w[e];
   }
-  u64 mi = wave_scan64(own, lane);
+  u64 mi = wave_scan64(own);
   if (lane == 63) S.part[wave] = mi;
   __syncthreads();
   u64 here = before;
-  for (int x = 0; x < wave; ++x) here += S.part[x];
+#pragma unroll
+  for (int x = 0; x < ST / 64; ++x) here += x < wave ? S.part[x] : 0;
   mi += here;
   // one thread's values hold the target: the first whose sum passes it, or past the end the last with any mass
   bool mine;
@@ -1099,10 +1121,10 @@ static SamplePlan sample_plan(const fa_sample_args* ap) {
   FA_REQUIRE(a.row_stride >= a.vocab || a.rows <= 1, "sample_tokens: rows overlap");
   int lg = 0;
   while ((1 << lg) < a.vocab) ++lg;
-  t.P.one = (double)(1ull << (62 - lg));
-  // 256 threads a block where that still leaves the launch at up to four blocks a compute unit, else 1024
+  t.P.S = std::min(50, 62 - lg);  // the whole row's sum stays below 2^62
+  // 256 threads a block up to 8192 blocks (and 1024 chunks, a thread of k_finish each), else 1024
   const int64_t small = (a.vocab + PER * 256 - 1) / (PER * 256);
-  t.bt = a.rows * small <= 1024 ? 256 : 1024;
+  t.bt = a.rows * small <= 8192 && small <= ST ? 256 : 1024;
   t.P.chunks = (a.vocab + PER * t.bt - 1) / (PER * t.bt);
   t.P.hist_chunks = (a.vocab + PER * ST - 1) / (PER * ST);
   FA_REQUIRE((int64_t)a.rows * t.P.chunks < (1ll << 31), "sample_tokens: more than 2^31 chunks");
