@@ -82,4 +82,22 @@ inline int cu_count() {
   return n;
 }
 
+// The operators themselves (the C entries fa_qk_norm_rope .. fa_sample_tokens without their error frame), for the engine's
+// own steps.
+void head_rows(const fa_head_rows_args* a, bool cache, hipStream_t s);  // cache: fa_kv_append, else fa_qk_norm_rope
+int64_t tree_attention_bytes(const fa_tree_attention_args* a);
+void tree_attention(const fa_tree_attention_args* a, hipStream_t s);
+int64_t sample_tokens_bytes(const fa_sample_args* a);
+void sample_tokens(const fa_sample_args* a, hipStream_t s);
+// rows base + path[i] of every head move to base + i (i = 1 .. n - 1; path rises, path[i] >= i) in `caches` caches of `heads`
+// heads each: cache c, head h at p[c / per_ptr] + (c % per_ptr) * cache_stride + h * head_stride
+struct KeepPath {
+  static constexpr int MAX = 64;
+  _Float16* p[2];
+  int64_t cache_stride, head_stride;
+  int per_ptr, head_dim, n;
+  int16_t path[MAX];
+};
+void keep_path(const KeepPath& k, int heads, hipStream_t s);
+
 }  // namespace fa

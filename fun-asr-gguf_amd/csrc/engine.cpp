@@ -20,6 +20,7 @@
 #include "../../include/funasr_hip.h"
 #include "api.h"
 #include "common.h"
+#include "draft_ops.h"
 #include "gguf.h"
 #include "kernels.h"
 
@@ -124,6 +125,13 @@ struct Engine {
   int64_t prow_cap = 0;
   int* d_rowsrc = nullptr;     // fa_llm_prefill_rows: row codes of one forward
   std::vector<int> h_tlfr, h_tgt, h_ctclen;
+  // verification of drafted tokens (fa_llm_verify); the buffers exist from the first call on
+  static constexpr int VF_MAX = fa::KeepPath::MAX;  // rows of one forward: the token to feed and its drafts
+  int vf_rows = 0, vf_seq = 0;                      // the verifying forward being run (0 rows: none)
+  float *vf_logits = nullptr, *vf_pval = nullptr;
+  int *vf_pidx = nullptr, *vf_meta = nullptr;       // meta: tokens, positions, slots, u, drawn, seq, n_past, mask
+  char* vf_ws = nullptr;                            // workspace of tree_attention / sample_tokens, one after the other
+  int64_t vf_ws_cap = 0;
 
   // decoder
   std::vector<LlmLayerW> layers;
@@ -251,6 +259,7 @@ struct Engine {
     if (hp_rowsrc) hipHostFree(hp_rowsrc);
     if (ev_rowsrc) hipEventDestroy(ev_rowsrc);
     if (d_prow) hipFree(d_prow);
+    if (vf_ws) hipFree(vf_ws);
     for (auto& l : enc_lanes)
       if (l.s) hipStreamSynchronize(l.s);
     if (stream) hipStreamSynchronize(stream);
@@ -1352,11 +1361,13 @@ struct Engine {
       if (!ob) {
         hipEvent_t ev;
         prof_begin(3, &ev);
-        if (!decode)
+        if (!decode && !vf_rows)
           qk_rope_store(lqkv, M, H, KV, lc.rms_eps, w.q_norm, w.k_norm, rcos, rsin, d_tok_seq, d_tok_pos, lq, kc, vc,
                         seq_stride, stream);
         // M > 4: the attention also leaves its rows as q8_0 blocks for the o GEMM (no prep launch)
-        if (!decode && n_ptiles > 0)  // query tiles: each K/V tile serves 64 rows x 2 heads (set_prefill_tiles)
+        if (vf_rows)
+          verify_attention(w, kc, vc, small);
+        else if (!decode && n_ptiles > 0)  // query tiles: each K/V tile serves 64 rows x 2 heads (set_prefill_tiles)
           attn_prefill(d_ptiles, n_ptiles, d_tok_pos, H, KV, seq_stride, kc, vc, lq, latt, small ? nullptr : lxq2,
                        small ? nullptr : lxd2, stream, ptiles_f16);
         else
@@ -1408,8 +1419,8 @@ struct Engine {
     prof_layer0 = prof_prefill = false;
     // lm_head (tied token_embd) with fused argmax partials: all rows (decode), the last row (prefill) or each
     // sequence's last row (prefill batch)
-    const int n_rows = decode ? M : n_last > 0 ? n_last : 1;
-    const float* xrow = decode ? lx : lx + (size_t)(M - 1) * E;
+    const int n_rows = decode || vf_rows ? M : n_last > 0 ? n_last : 1;
+    const float* xrow = decode || vf_rows ? lx : lx + (size_t)(M - 1) * E;
     if (!decode && n_last > 0) {
       gather_rows(lx, d_lastrow, n_last, E, lxg, stream);
       xrow = lxg;
@@ -1419,6 +1430,7 @@ struct Engine {
     h.rpw = gemv_rows_per_wave(lc.n_vocab);
     h.out = logits; h.ldo = lc.n_vocab;
     h.pval = pval; h.pidx = pidx; h.n_part = n_part_cur = lm_head_parts(lc.n_vocab, n_rows, E);
+    if (vf_rows) { h.out = vf_logits; h.pval = vf_pval; h.pidx = vf_pidx; }
     chunk_cur = lm_head_chunk(lc.n_vocab, n_rows, E);
     if (gemv_small(n_rows)) { h.x = xrow; h.ldx = E; h.norm_w = out_norm; }
     else if (nrm) { h.xq = lxq; h.xd = lxd; h.ssp = d_ssp; }  // rows from the last down epilogue
@@ -1687,6 +1699,158 @@ struct Engine {
     std::fill(logits_row.begin(), logits_row.end(), -1);
     logits_row[seq] = 0;
     if (tok_out) *tok_out = tok;
+  }
+
+  // ---- verification of drafted tokens (fa_llm_verify)
+  // byte offsets of vf_meta
+  static constexpr int VF_POS = VF_MAX * 4, VF_SLOT = VF_MAX * 8, VF_U = VF_MAX * 12, VF_SEQ = VF_MAX * 16,
+                       VF_MASK = VF_MAX * 16 + 16, VF_BYTES = VF_MASK + VF_MAX * VF_MAX;
+  template <class T>
+  T* vf_at(int byte) { return reinterpret_cast<T*>(reinterpret_cast<char*>(vf_meta) + byte); }
+
+  void vf_reserve(int64_t bytes) {
+    if (bytes <= vf_ws_cap) return;
+    if (vf_ws) FA_HIP(hipFree(vf_ws));
+    vf_ws = nullptr;
+    vf_ws_cap = 0;
+    FA_HIP(hipMalloc(&vf_ws, (size_t)bytes));
+    vf_ws_cap = bytes;
+  }
+
+  // the decoder's cache as pages: a sequence is one page of n_ctx rows
+  fa_tree_attention_args vf_attention_args(int M) const {
+    const int H = lc.n_head, KV = lc.n_head_kv, D = lc.head_dim;
+    fa_tree_attention_args t{};
+    t.q_node = t.out_node = (int64_t)H * D;
+    t.q_seq = t.out_seq = t.q_node * M;
+    t.q_head = t.out_head = D;
+    t.k_page = t.v_page = seq_stride;
+    t.k_head = t.v_head = (int64_t)lc.n_ctx * D;
+    t.k_slot = t.v_slot = D;
+    t.table_seq = 1; t.mask_seq = 0; t.mask_row = M;
+    t.seqs = 1; t.nodes = M; t.heads = H; t.kv_heads = KV; t.head_dim = D;
+    t.q_type = FA_F32; t.cache_type = FA_F16;
+    t.pages = lc.max_seqs; t.page_size = lc.n_ctx; t.table_len = 1;
+    t.max_context = n_past[vf_seq];
+    t.scale = (float)(1.0 / std::sqrt((double)D));
+    return t;
+  }
+
+  // one layer's attention over the cache for the drafted rows of lqkv: head norms, rotation and append in one launch, then
+  // the tree's attention; its rows to latt, or as q8_0 blocks for the o GEMM
+  void verify_attention(const LlmLayerW& w, __half* kc, __half* vc, bool small) {
+    const int M = vf_rows, H = lc.n_head, KV = lc.n_head_kv, D = lc.head_dim, QKV = (H + 2 * KV) * D;
+    fa_head_rows_args r{};
+    r.q = lqkv; r.k = lqkv + H * D; r.v = lqkv + (H + KV) * D;
+    r.q_out = lq; r.k_out = kc; r.v_out = vc;
+    r.q_weight = w.q_norm; r.k_weight = w.k_norm; r.cos = rcos; r.sin = rsin;
+    r.positions = vf_at<int>(VF_POS); r.slots = vf_at<int>(VF_SLOT);
+    r.q_token = r.k_token = r.v_token = QKV;
+    r.q_head = r.k_head = r.v_head = D;
+    r.q_out_token = (int64_t)H * D; r.q_out_head = D;
+    r.k_out_token = r.v_out_token = D; r.k_out_head = r.v_out_head = (int64_t)lc.n_ctx * D;
+    r.k_out_page = r.v_out_page = seq_stride;
+    r.tokens = M; r.heads = H; r.kv_heads = KV; r.head_dim = r.rot_dim = D; r.table_len = lc.n_ctx;
+    r.type = FA_F32; r.cache_type = FA_F16;
+    r.pages = lc.max_seqs; r.page_size = lc.n_ctx;
+    r.eps = lc.rms_eps;
+    head_rows(&r, true, stream);
+    fa_tree_attention_args t = vf_attention_args(M);
+    t.q = lq; t.out = latt; t.k_cache = kc; t.v_cache = vc;
+    t.block_table = vf_at<int>(VF_SEQ); t.context_lens = vf_at<int>(VF_SEQ + 4);
+    t.mask = vf_at<uint8_t>(VF_MASK);
+    t.workspace = vf_ws; t.workspace_bytes = vf_ws_cap;
+    tree_attention(&t, stream);
+    if (!small) prep_q8(latt, (int64_t)H * D, nullptr, lc.rms_eps, M, H * D, lxq2, lxd2, stream);
+  }
+
+  // the drafts' forward, a draw at every row, the longest accepted path and its rows in the cache; returns the tokens gained
+  int verify(int seq, const int32_t* tokens, const int32_t* parents, int n, const fa_sampling* s, const float* u,
+             int32_t* tokens_out, int32_t* path_out) {
+    const int M = n + 1, E = lc.n_embd, V = lc.n_vocab;
+    if (!vf_meta) {
+      vf_logits = alloc<float>((size_t)VF_MAX * V);
+      vf_pval = alloc<float>((size_t)VF_MAX * n_part);
+      vf_pidx = alloc<int>((size_t)VF_MAX * n_part);
+      vf_meta = alloc<int>(VF_BYTES / 4);
+    }
+    vf_seq = seq;
+    fa_sample_args a{};
+    a.logits = vf_logits;
+    a.u = vf_at<float>(VF_U);
+    a.token_out = vf_at<int>(0);  // over the rows' own tokens, which the embedding has read
+    a.row_stride = V; a.rows = M; a.vocab = V; a.type = FA_F32;
+    a.top_k = s ? s->top_k : 0; a.temperature = s ? s->temperature : 0.f; a.top_p = s ? s->top_p : 1.f;
+    const fa_tree_attention_args t = vf_attention_args(M);
+    vf_reserve(std::max(tree_attention_bytes(&t), sample_tokens_bytes(&a)));
+    a.workspace = vf_ws; a.workspace_bytes = vf_ws_cap;
+
+    std::vector<char> meta(VF_BYTES, 0);
+    int* const tok = reinterpret_cast<int*>(meta.data());
+    int* const pos = reinterpret_cast<int*>(meta.data() + VF_POS);
+    int* const slot = reinterpret_cast<int*>(meta.data() + VF_SLOT);
+    float* const uu = reinterpret_cast<float*>(meta.data() + VF_U);
+    int* const sq = reinterpret_cast<int*>(meta.data() + VF_SEQ);
+    char* const mask = meta.data() + VF_MASK;
+    for (int i = 0; i < M; ++i) {
+      const int parent = i ? parents ? parents[i - 1] + 1 : i - 1 : -1;
+      tok[i] = i ? tokens[i - 1] : last_tok[seq];
+      pos[i] = i ? pos[parent] + 1 : n_past[seq];
+      slot[i] = seq * lc.n_ctx + n_past[seq] + i;
+      uu[i] = u ? u[i] : 0.f;
+      if (i) std::memcpy(mask + i * M, mask + parent * M, M);
+      mask[i * M + i] = 1;
+    }
+    sq[0] = seq;
+    sq[1] = n_past[seq];
+    std::vector<int> own(tok, tok + M);
+    FA_HIP(hipMemcpyAsync(vf_meta, meta.data(), meta.size(), hipMemcpyHostToDevice, stream));
+    fa::embed_rows(tok_embd.q, tok_embd.d, vf_at<int>(0), M, E, 0, lx, stream);
+    // (the GEMVs up to g_gemv_small_max rows, the split-K GEMMs above, as a decode batch: full model, 300 tokens, 1 / 4 / 8 /
+    // 64 rows 1.00 / 1.22 / 1.53 / 2.12 ms; on the row-local GEMMs of a prompt 1.83 / 1.88 / 1.94 / 2.66 ms)
+    vf_rows = M;
+    try {
+      llm_forward(M, false, n_past[seq] + M - 1);
+    } catch (...) {
+      vf_rows = 0;
+      throw;
+    }
+    vf_rows = 0;
+    sample_tokens(&a, stream);
+    std::vector<int> drawn(M);
+    FA_HIP(hipMemcpyAsync(drawn.data(), vf_at<int>(0), (size_t)M * 4, hipMemcpyDeviceToHost, stream));
+    FA_HIP(hipStreamSynchronize(stream));
+    prof_collect();
+
+    fa::KeepPath k{};
+    int at = 0;
+    bool moved = false;
+    for (;;) {
+      FA_REQUIRE(drawn[at] >= 0, "fa_llm_verify: no logit is above -inf");
+      if (path_out && at) path_out[k.n - 1] = at - 1;
+      moved |= at != k.n;
+      tokens_out[k.n] = drawn[at];
+      k.path[k.n++] = (int16_t)at;
+      int next = 0;
+      for (int i = at + 1; i < M && !next; ++i)
+        if ((parents ? parents[i - 1] + 1 : i - 1) == at && own[i] == drawn[at]) next = i;
+      if (!next) break;
+      at = next;
+    }
+    if (moved) {
+      const int64_t base = (int64_t)seq * seq_stride + (int64_t)n_past[seq] * lc.head_dim;
+      k.p[0] = reinterpret_cast<_Float16*>(kcache) + base;
+      k.p[1] = reinterpret_cast<_Float16*>(vcache) + base;
+      k.cache_stride = layer_stride; k.head_stride = (int64_t)lc.n_ctx * lc.head_dim;
+      k.per_ptr = lc.n_layer; k.head_dim = lc.head_dim;
+      keep_path(k, lc.n_head_kv, stream);
+    }
+    FA_HIP(hipMemcpyAsync(logits, vf_logits + (int64_t)at * V, (size_t)V * 4, hipMemcpyDeviceToDevice, stream));
+    n_past[seq] += k.n;
+    last_tok[seq] = drawn[at];
+    std::fill(logits_row.begin(), logits_row.end(), -1);
+    logits_row[seq] = 0;
+    return k.n;
   }
 
   // one decode step for the n active sequences: embed last token -> forward -> sample -> advance
@@ -2533,6 +2697,29 @@ int fa_llm_generate(fa_engine* h, const int32_t* seqs, int32_t n_seqs, int32_t n
   const int rc = fa_llm_generate_begin(h, seqs, n_seqs, n_steps, s);
   if (rc != FA_OK) return rc;
   return fa_llm_generate_end(h, tokens_out);
+}
+
+int fa_llm_verify(fa_engine* h, int32_t seq, const int32_t* tokens, const int32_t* parents, int32_t n, const fa_sampling* s,
+                  const float* u, int32_t* tokens_out, int32_t* path_out, int32_t* n_out) {
+  FA_API_BEGIN
+  FA_REQUIRE(h && tokens_out && n_out, "fa_llm_verify: arguments");
+  Engine* e = h->e;
+  FA_REQUIRE(!e->gen_pending, "a generate call is in flight (fa_llm_generate_end first)");
+  FA_REQUIRE(seq >= 0 && seq < e->lc.max_seqs, "seq out of range");
+  FA_REQUIRE(n >= 0 && n < Engine::VF_MAX && (tokens || n == 0), "fa_llm_verify: 0 to 63 drafted tokens");
+  FA_REQUIRE(e->last_tok[seq] >= 0, "sequence has no sampled token (prefill first)");
+  FA_REQUIRE(e->n_past[seq] + n + 1 <= e->lc.n_ctx, "verify exceeds n_ctx");
+  for (int i = 0; i < n; ++i) {
+    FA_REQUIRE(tokens[i] >= 0 && tokens[i] < e->lc.n_vocab, "fa_llm_verify: token out of range");
+    FA_REQUIRE(!parents || (parents[i] >= -1 && parents[i] < i), "fa_llm_verify: a parent stands before its child");
+  }
+  if (s) {
+    FA_REQUIRE(s->temperature == s->temperature && s->top_p == s->top_p, "sampling: NaN parameter");
+    FA_REQUIRE(u || !(s->temperature > 0.f), "fa_llm_verify: drawing needs the random numbers");
+  }
+  for (int i = 0; u && i <= n; ++i) FA_REQUIRE(u[i] >= 0.f && u[i] < 1.f, "fa_llm_verify: u lies in [0, 1)");
+  *n_out = e->verify(seq, tokens, parents, n, s, u, tokens_out, path_out);
+  FA_API_END
 }
 
 int fa_llm_invariant_width(fa_engine* h, int32_t* out) {

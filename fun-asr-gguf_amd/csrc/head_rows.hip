@@ -133,7 +133,7 @@ static bool rows_aligned(const void* p, int64_t st, int64_t sh, int type) {
   return !p || (aligned16(p) && st % m == 0 && sh % m == 0);
 }
 
-static void head_rows(const fa_head_rows_args* ap, bool cache, hipStream_t s) {
+void head_rows(const fa_head_rows_args* ap, bool cache, hipStream_t s) {
   FA_REQUIRE(ap, "head rows: no arguments");
   HeadRowsP P;
   P.a = *ap;
@@ -200,6 +200,24 @@ static void head_rows(const fa_head_rows_args* ap, bool cache, hipStream_t s) {
     if (a.cache_type == FA_BF16) head_rows_launch<__bf16, __bf16>(P, vec, s);
     else head_rows_launch<__bf16, _Float16>(P, vec, s);
   }
+}
+
+// The accepted drafts of one sequence close up behind its committed tokens. A thread holds the same 16 bytes of every row, in
+// order, so a row is read before anything is written over it: row i is the source of an earlier step only (path[j] = i
+// needs j <= i). At most 63 rows of 256 bytes a head; the launch is what it costs.
+__global__ __launch_bounds__(64) void k_keep_path(KeepPath k) {
+  _Float16* const p = k.p[blockIdx.y / k.per_ptr] + (int64_t)(blockIdx.y % k.per_ptr) * k.cache_stride + blockIdx.x * k.head_stride;
+  for (int d = threadIdx.x * 8; d < k.head_dim; d += 64 * 8)
+    for (int i = 1; i < k.n; ++i)
+      if (k.path[i] != i)
+        *reinterpret_cast<f16x8_t*>(p + (int64_t)i * k.head_dim + d) =
+            *reinterpret_cast<const f16x8_t*>(p + (int64_t)k.path[i] * k.head_dim + d);
+}
+
+void keep_path(const KeepPath& k, int heads, hipStream_t s) {
+  FA_REQUIRE(k.n >= 1 && k.n <= KeepPath::MAX && k.head_dim % 8 == 0 && k.per_ptr >= 1, "keep_path: sizes");
+  for (int i = 1; i < k.n; ++i) FA_REQUIRE(k.path[i] > k.path[i - 1] && k.path[i] < KeepPath::MAX, "keep_path: path");
+  launch(k_keep_path, dim3(heads, 2 * k.per_ptr), dim3(64), 0, s, k);
 }
 
 }  // namespace fa

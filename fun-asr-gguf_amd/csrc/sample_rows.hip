@@ -1169,7 +1169,9 @@ static void sample_run(const SamplePlan& t, hipStream_t s) {
   go(k_finish<T, BT>, 1, ST);
 }
 
-static void sample_tokens(const fa_sample_args* ap, hipStream_t s) {
+int64_t sample_tokens_bytes(const fa_sample_args* a) { return sample_plan(a).bytes; }
+
+void sample_tokens(const fa_sample_args* ap, hipStream_t s) {
   const SamplePlan t = sample_plan(ap);
   const fa_sample_args& a = t.P.a;
   if (a.rows == 0) return;
@@ -1188,7 +1190,7 @@ extern "C" {
 int fa_sample_tokens_workspace(const fa_sample_args* a, int64_t* bytes) {
   FA_API_BEGIN
   FA_REQUIRE(bytes, "sample_tokens: no place for the size");
-  *bytes = fa::sample_plan(a).bytes;
+  *bytes = fa::sample_tokens_bytes(a);
   FA_API_END
 }
 

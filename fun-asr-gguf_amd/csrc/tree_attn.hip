@@ -756,9 +756,9 @@ static TreePlan tree_plan(const fa_tree_attention_args* ap) {
   t.P.splits = 1;
   t.P.chunk = 1 << 30;
   if (a.seqs == 0 || a.nodes == 0) return t;
-  // The keys are split w ways so that rounds(w) (keys / w + 256), and 300 for the launch that joins them, is least: two blocks a
-  // compute unit are resident at once, and a block's beginning and end weigh about as much as 256 keys. (32 sequences of up to 2048 keys on 8 kv heads: 2 ways 50 us, 3:
-  // 60, 1: 57; 4 long ones with two row tiles: 8 ways 241 us, 16: 258.)
+  // The keys are split w ways so that rounds(w) (keys / w + 256), and 300 for the launch that joins them, is least: two blocks
+  // a compute unit are resident at once, and a block's beginning and end weigh about as much as 256 keys. (32 sequences of up
+  // to 2048 keys on 8 kv heads: 2 ways 50 us, 3: 60, 1: 57; 4 long ones with two row tiles: 8 ways 241 us, 16: 258.)
   const int64_t cap = (int64_t)a.table_len * a.page_size;
   const int64_t keys = std::max<int64_t>(1, std::min<int64_t>(cap, a.max_context > 0 ? (int64_t)a.max_context + a.nodes : cap));
   const int64_t base = (int64_t)a.seqs * a.kv_heads * t.P.q_tiles, slots = 2ll * cu_count();
@@ -832,7 +832,9 @@ static void tree_dispatch(const TreePlan& t, hipStream_t s) {
   else tree_run<T, NS, 256>(t, s);
 }
 
-static void tree_attention(const fa_tree_attention_args* ap, hipStream_t s) {
+int64_t tree_attention_bytes(const fa_tree_attention_args* a) { return tree_plan(a).bytes; }
+
+void tree_attention(const fa_tree_attention_args* ap, hipStream_t s) {
   TreePlan t = tree_plan(ap);
   const fa_tree_attention_args& a = t.P.a;
   if (a.seqs == 0 || a.nodes == 0) return;
@@ -871,7 +873,7 @@ extern "C" {
 int fa_tree_attention_workspace(const fa_tree_attention_args* a, int64_t* bytes) {
   FA_API_BEGIN
   FA_REQUIRE(bytes, "tree_attention: no place for the size");
-  *bytes = fa::tree_plan(a).bytes;
+  *bytes = fa::tree_attention_bytes(a);
   FA_API_END
 }
 

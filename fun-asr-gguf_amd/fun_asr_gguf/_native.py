@@ -23,7 +23,7 @@ EXPORTS = [
     "fa_weights_mark_unset", "fa_tensor_names", "fa_llm_set_token",
     "fa_llm_invariant_width", "fa_set_encode_mode", "fa_ctc_head", "fa_set_tensor_u8dq", "fa_set_ctc_int8",
     "fa_ctc_int8_active", "fa_comm_unique_id", "fa_comm_init", "fa_comm_allgather_sizes", "fa_comm_allgather_bytes",
-    "fa_comm_destroy", "fa_llm_prefill_rows", "fa_encode_generation", "fa_llm_decode_recoveries",
+    "fa_comm_destroy", "fa_llm_prefill_rows", "fa_encode_generation", "fa_llm_decode_recoveries", "fa_llm_verify",
     "fa_qk_norm_rope", "fa_kv_append", "fa_tree_attention", "fa_tree_attention_workspace", "fa_sample_tokens",
     "fa_sample_tokens_workspace",
 ]
@@ -135,6 +135,7 @@ def load():
     lib.fa_llm_prefill_batch.argtypes = [P, P, I32, P, P, ctypes.POINTER(Sampling), P]
     lib.fa_llm_prefill_rows.argtypes = [P, P, I32, P, I32, P, P, I64, ctypes.POINTER(Sampling), P]
     lib.fa_encode_generation.argtypes = [P, P]
+    lib.fa_llm_verify.argtypes = [P, I32, P, P, I32, ctypes.POINTER(Sampling), P, P, P, P]
     lib.fa_llm_logits.argtypes = [P, I32, P]
     lib.fa_llm_set_token.argtypes = [P, I32, I32]
     lib.fa_llm_invariant_width.argtypes = [P, ctypes.c_void_p]
@@ -496,6 +497,21 @@ class Engine:
         out = np.empty(self._gen_shape, np.int32)
         _check(self.lib.fa_llm_generate_end(self.h, _ptr(out)), "fa_llm_generate_end")
         return out
+
+    def llm_verify(self, seq, tokens, parents=None, u=None, **samp):
+        """One decode step that also verifies drafted tokens (fa_llm_verify): a tree below the token that the next step would
+        feed, parents[i] < i the index of draft i's parent or -1 (None: a chain). u: len(tokens) + 1 random numbers in [0, 1),
+        needed with a temperature. -> (tokens gained, the accepted drafts' indices)."""
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        p = None if parents is None else np.ascontiguousarray(parents, dtype=np.int32)
+        r = None if u is None else np.ascontiguousarray(u, dtype=np.float32)
+        if t.ndim != 1 or (p is not None and p.shape != t.shape) or (r is not None and r.shape != (t.size + 1,)):
+            raise ValueError("llm_verify: tokens [n], parents [n], u [n + 1]")
+        out, path, n = np.empty(t.size + 1, np.int32), np.empty(t.size, np.int32), ctypes.c_int32()
+        s = self._sampling(**samp)
+        _check(self.lib.fa_llm_verify(self.h, seq, _ptr(t), _ptr(p), t.size, ctypes.byref(s), _ptr(r), _ptr(out), _ptr(path),
+                                      ctypes.byref(n)), "fa_llm_verify")
+        return out[:n.value].tolist(), path[:n.value - 1].tolist()
 
     def llm_invariant_width(self):
         """Largest decode batch width with single-sequence arithmetic per token (fa_llm_invariant_width)."""

@@ -6,15 +6,24 @@ gfx950 kernels on the current stream of their tensors' device, allocate nothing 
 allocator, on that stream), never synchronise, and can be captured into a graph. A tensor that was made on another stream is
 ordered before the call by its user, as with any torch operation. Wrong shapes, types, strides or devices raise ValueError
 before anything is enqueued; a refusal of the library raises RuntimeError with its message. There is no CPU fallback.
+
+A program that also creates an Engine imports torch (or this module) before the first one: torch brings a HIP runtime of its
+own, and the engine's library uses it where it is loaded already. The other way round the process holds two, and torch's
+finds no device.
 """
 import ctypes
 import importlib.machinery
 import importlib.util
 import os
-
-import torch
+import sys
+import warnings
 
 from . import _native
+
+if _native._lib is not None and "torch" not in sys.modules:
+    warnings.warn("torch is imported after the engine's library has loaded another HIP runtime and will find no GPU: import "
+                  "torch or fun_asr_gguf.ops before the first Engine", RuntimeWarning, stacklevel=2)
+import torch  # noqa: E402
 
 _BINDING = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lib", "draft_ops.so")
 _module = None

@@ -201,6 +201,17 @@ int fa_llm_generate_end(fa_engine* e, int32_t* tokens_out);
 /* (fa_llm_generate_end: when the chunk ran on the fused small-batch layer and one of its in-launch fan-ins timed out --
  * a group of blocks not co-resident because another kernel held CUs -- the chunk is decoded again on the 5-launch layer
  * from the same positions and input tokens, and the engine keeps that layer; the tokens returned are the re-run's.) */
+/* One decode step of sequence `seq` that also verifies n drafted tokens (0 .. 63), a tree whose root is the token that a
+ * generate step would feed next: parents[i] is the index of draft i's parent, below i, or -1 for that token (NULL: a
+ * chain). One forward over the n + 1 rows (fa_kv_append and fa_tree_attention on the engine's cache) gives every row its
+ * next-token logits, and fa_sample_tokens draws from each with `s` (its seed is not used; NULL or temperature <= 0: the
+ * largest logit) and u[row] in [0, 1), u [n + 1], row 0 the root's. From the root on, while a child holds the token drawn at
+ * its parent, it is accepted. tokens_out [n + 1] receives the *n_out tokens drawn along the accepted path (at least one;
+ * the last is what the next step feeds), path_out [n] (nullable) the accepted drafts' indices (*n_out - 1 of them). The
+ * cache keeps the accepted rows alone, so the sequence goes on as if these tokens had been generated one by one: to the
+ * decoder's noise floor, not bit for bit (other f32 summation orders). */
+int fa_llm_verify(fa_engine* e, int32_t seq, const int32_t* tokens, const int32_t* parents, int32_t n, const fa_sampling* s,
+                  const float* u, int32_t* tokens_out, int32_t* path_out, int32_t* n_out);
 /* Logits [n_vocab] of sequence `seq` from the most recent forward (fa_llm_prefill, or the last step of
  * fa_llm_generate) when that forward included it; FA_ERR_ARG otherwise (test hook; llama_get_logits_ith). */
 int fa_llm_logits(fa_engine* e, int32_t seq, float* out);

@@ -3,6 +3,8 @@ fa_sample_tokens with sizes, strides, types and pointers that do not fit), what 
 forms the GPU tests compare with."""
 import ctypes
 
+import os
+
 import numpy as np
 import pytest
 import torch
@@ -141,3 +143,15 @@ def test_plain_forms():
     assert sample(z, 0.99, 1.0, 3, 1.0, 0.0)[0] == 2 and sample(z, 0.99, 1.0, 0, 0.79, 0.0)[0] == 1
     assert sample(z, 0.99, 1.0, 0, 1.0, 0.25)[0] == 2 and sample(z, 0.99, 0.0, 0, 1.0, 0.0)[:2] == (0, 1.0)
     assert sample([1.0, 2.0, 2.0, 2.0], 0.99, 1.0, 2, 1.0, 0.0)[0] == 2  # equal values: the lower ids
+
+
+@pytest.mark.parametrize("first,warned", [("fun_asr_gguf._native as n; n.load()", True), ("torch", False)])
+def test_import_order(first, warned):
+    """torch behind the engine's library in one process would find no GPU: importing the operators says so."""
+    import subprocess
+    import sys
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fun-asr-gguf_amd")
+    prog = f"import sys; sys.path.insert(0, {pkg!r})\nimport {first}\nimport fun_asr_gguf._native as n; n.load()\nimport fun_asr_gguf.ops"
+    r = subprocess.run([sys.executable, "-W", "always", "-c", prog], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    assert ("before the first Engine" in r.stderr) == warned

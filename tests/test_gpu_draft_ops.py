@@ -11,6 +11,7 @@ Tolerances, from arithmetic (u = half a step of the output's type relative to th
 """
 import numpy as np
 import pytest
+import torch  # noqa: F401  (before any engine: the library then shares torch's HIP runtime)
 
 from draft_oracle import attention, norm_rope, sample
 
