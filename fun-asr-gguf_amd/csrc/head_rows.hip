@@ -3,10 +3,13 @@
 // Per head row x of head_dim D: y = x * rsqrt(mean x^2 + eps) * w, then the pairs of the first R dimensions turned by the
 // token's angles. Each row is read once and written once, with one pass of arithmetic in between: memory bound.
 //
-// A row is held by a group of LPR lanes (the power of two >= D / 16), two runs of 8 elements a lane: the two halves of its
-// own 8 pairs, so that the rotation needs no exchange between lanes. Half-split pairs (i, i + R/2): runs at 8 p and
-// R/2 + 8 p; neighbouring pairs, and the dimensions behind R: runs at 16 p and 16 p + 8. The sum of squares is the only
-// thing the lanes share (log2 LPR exchanges). A wave thus moves 64 / LPR rows with 16-byte accesses.
+// A row is held by a group of D / 16 lanes, two runs of 8 elements a lane: the two halves of its own 8 pairs, so that the
+// rotation needs no exchange between lanes. Half-split pairs (i, i + R/2): runs at 8 p and R/2 + 8 p; neighbouring pairs, and
+// the dimensions behind R: runs at 16 p and 16 p + 8. The sum of squares is the only thing the lanes share. A wave thus moves
+// floor(64 / (D / 16)) rows with 16-byte accesses (heads of 80 in groups of eight lanes, three idle: 45.6 us, of five: 40.3).
+// Several rows of a token in one group, to read its angles once, cost registers and bring nothing (24 f32 heads of 128: four
+// rows 35 us, one 31). Measured: 6528 tokens of 16 + 8 f32 heads of 128 31 us, 5.2 TB/s read and written; one token 2.9 us, the
+// launch; 16384 tokens of 8 + 8 bf16 heads of 64 appended 15 us, 4.8 TB/s.
 #include "api.h"
 #include "draft_ops.h"
 
@@ -14,13 +17,13 @@ namespace fa {
 
 struct HeadRowsP {
   fa_head_rows_args a;
-  FastDiv slots_div;  // by head slots of a unit
+  FastDiv slots_div;  // by n_slots
   FastDiv page_div;
-  int lpr_log;        // log2 lanes per row
+  FastDiv lpr_div;    // by the lanes of a row
+  uint32_t lpr, wave_rows;  // lanes of a row, rows of a wave
+  float inv_dim;
   int n_slots;        // head rows per token: heads + kv_heads (+ kv_heads of v)
-  int per_unit;       // rows of one token a group of lanes makes one after the other (its angles stay in registers)
-  int units_per_token;
-  uint32_t n_units;
+  uint32_t n_rows;
 };
 
 __device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
@@ -30,13 +33,12 @@ __device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) 
 template <typename TI, typename TC, bool VEC>
 __global__ __launch_bounds__(256) void k_head_rows(HeadRowsP P) {
   const fa_head_rows_args& a = P.a;
-  const uint32_t unit = blockIdx.x * (256u >> P.lpr_log) + (threadIdx.x >> P.lpr_log);
-  if (unit >= P.n_units) return;
-  const int p = threadIdx.x & ((1 << P.lpr_log) - 1);
-  const int t = (int)P.slots_div.div(unit);
-  const int s0 = (int)(unit - (uint32_t)t * P.units_per_token);
-  const int D = a.head_dim, R = a.rot_dim;
-  const bool in = 16 * p < D;
+  const uint32_t lane = threadIdx.x & 63, group = P.lpr_div.div(lane);
+  const uint32_t row = (blockIdx.x * 4 + (threadIdx.x >> 6)) * P.wave_rows + group;
+  if (group >= P.wave_rows || row >= P.n_rows) return;
+  const int p = (int)(lane - group * P.lpr);
+  const int t = (int)P.slots_div.div(row), s = (int)(row - (uint32_t)t * P.n_slots);
+  const int R = a.rot_dim;
   const bool rot = a.cos && 16 * p < R;
   const bool halves = rot && !a.interleaved;
   const int e0 = halves ? 8 * p : 16 * p, e1 = halves ? R / 2 + 8 * p : 16 * p + 8;
@@ -57,74 +59,71 @@ __global__ __launch_bounds__(256) void k_head_rows(HeadRowsP P) {
       off = slot - page * a.page_size;
     }
   }
-  for (int j = 0, s = s0; j < P.per_unit && s < P.n_slots; ++j, s += P.units_per_token) {
-    const bool is_q = s < a.heads, is_v = s >= a.heads + a.kv_heads;
-    const int h = is_q ? s : is_v ? s - a.heads - a.kv_heads : s - a.heads;
-    if (!is_q && a.slots && page < 0) continue;  // a token without a slot is not appended
-    const TI* x = is_q ? reinterpret_cast<const TI*>(a.q) + t * a.q_token + h * a.q_head
-                  : is_v ? reinterpret_cast<const TI*>(a.v) + t * a.v_token + h * a.v_head
-                         : reinterpret_cast<const TI*>(a.k) + t * a.k_token + h * a.k_head;
-    float u[8] = {}, v[8] = {};
-    if (in) {
-      load8<VEC>(x + e0, u);
-      load8<VEC>(x + e1, v);
+  const bool is_q = s < a.heads, is_v = s >= a.heads + a.kv_heads;
+  const int h = is_q ? s : is_v ? s - a.heads - a.kv_heads : s - a.heads;
+  if (!is_q && a.slots && page < 0) return;  // a token without a slot is not appended
+  const TI* x = is_q ? reinterpret_cast<const TI*>(a.q) + t * a.q_token + h * a.q_head
+                : is_v ? reinterpret_cast<const TI*>(a.v) + t * a.v_token + h * a.v_head
+                       : reinterpret_cast<const TI*>(a.k) + t * a.k_token + h * a.k_head;
+  float u[8], v[8];
+  load8<VEC>(x + e0, u);
+  load8<VEC>(x + e1, v);
+  const float* w = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
+  if (w) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += u[i] * u[i] + v[i] * v[i];
+    // lane p holds the sum of lanes [p, p + 2 o) of its group, lane 0 in the end all of it
+    for (uint32_t o = 1; o < P.lpr; o <<= 1) {
+      const float other = __shfl(ss, lane + o);
+      if (p + o < P.lpr) ss += other;
     }
-    const float* w = is_q ? a.q_weight : is_v ? nullptr : a.k_weight;
-    if (w) {
-      float ss = 0.f;
+    ss = __shfl(ss, lane - p);
+    const float scale = rsqrtf(fmaf(ss, P.inv_dim, a.eps));
+    float wu[8], wv[8];
+    load8<VEC>(w + e0, wu);
+    load8<VEC>(w + e1, wv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += u[i] * u[i] + v[i] * v[i];
-      for (int o = 1; o < (1 << P.lpr_log); o <<= 1) ss += __shfl_xor(ss, o);
-      const float scale = 1.0f / sqrtf(ss / (float)D + a.eps);
-      if (in) {
-        float wu[8], wv[8];
-        load8<VEC>(w + e0, wu);
-        load8<VEC>(w + e1, wv);
+    for (int i = 0; i < 8; ++i) {
+      u[i] = u[i] * scale * wu[i];
+      v[i] = v[i] * scale * wv[i];
+    }
+  }
+  if (rot && !is_v) {
+    if (a.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          u[i] = u[i] * scale * wu[i];
-          v[i] = v[i] * scale * wv[i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float x0 = u[2 * i], y0 = u[2 * i + 1], x1 = v[2 * i], y1 = v[2 * i + 1];
+        u[2 * i] = x0 * c[i] - y0 * sn[i];
+        u[2 * i + 1] = x0 * sn[i] + y0 * c[i];
+        v[2 * i] = x1 * c[4 + i] - y1 * sn[4 + i];
+        v[2 * i + 1] = x1 * sn[4 + i] + y1 * c[4 + i];
       }
-    }
-    if (rot && !is_v) {
-      if (a.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x0 = u[2 * i], y0 = u[2 * i + 1], x1 = v[2 * i], y1 = v[2 * i + 1];
-          u[2 * i] = x0 * c[i] - y0 * sn[i];
-          u[2 * i + 1] = x0 * sn[i] + y0 * c[i];
-          v[2 * i] = x1 * c[4 + i] - y1 * sn[4 + i];
-          v[2 * i + 1] = x1 * sn[4 + i] + y1 * c[4 + i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x0 = u[i], y0 = v[i];
-          u[i] = x0 * c[i] - y0 * sn[i];
-          v[i] = x0 * sn[i] + y0 * c[i];
-        }
-      }
-    }
-    if (!in) continue;
-    if (is_q) {
-      TI* o = reinterpret_cast<TI*>(a.q_out) + t * a.q_out_token + h * a.q_out_head;
-      store8<VEC>(o + e0, u);
-      store8<VEC>(o + e1, v);
     } else {
-      TC* o = is_v ? reinterpret_cast<TC*>(a.v_out) + h * a.v_out_head : reinterpret_cast<TC*>(a.k_out) + h * a.k_out_head;
-      const int64_t st = is_v ? a.v_out_token : a.k_out_token;
-      o += a.slots ? page * (is_v ? a.v_out_page : a.k_out_page) + off * st : t * st;
-      store8<VEC>(o + e0, u);
-      store8<VEC>(o + e1, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x0 = u[i], y0 = v[i];
+        u[i] = x0 * c[i] - y0 * sn[i];
+        v[i] = x0 * sn[i] + y0 * c[i];
+      }
     }
+  }
+  if (is_q) {
+    TI* o = reinterpret_cast<TI*>(a.q_out) + t * a.q_out_token + h * a.q_out_head;
+    store8<VEC>(o + e0, u);
+    store8<VEC>(o + e1, v);
+  } else {
+    TC* o = is_v ? reinterpret_cast<TC*>(a.v_out) + h * a.v_out_head : reinterpret_cast<TC*>(a.k_out) + h * a.k_out_head;
+    const int64_t st = is_v ? a.v_out_token : a.k_out_token;
+    o += a.slots ? page * (is_v ? a.v_out_page : a.k_out_page) + off * st : t * st;
+    store8<VEC>(o + e0, u);
+    store8<VEC>(o + e1, v);
   }
 }
 
 template <typename TI, typename TC>
 static void head_rows_launch(const HeadRowsP& P, bool vec, hipStream_t s) {
-  const uint32_t per_block = 256u >> P.lpr_log;
-  const dim3 grid((P.n_units + per_block - 1) / per_block);
+  const dim3 grid((P.n_rows + 4 * P.wave_rows - 1) / (4 * P.wave_rows));
   launch(vec ? k_head_rows<TI, TC, true> : k_head_rows<TI, TC, false>, grid, dim3(256), 0, s, P);
 }
 
@@ -177,13 +176,12 @@ void head_rows(const fa_head_rows_args* ap, bool cache, hipStream_t s) {
              "head rows: k in place with other strides");
   FA_REQUIRE((int64_t)a.tokens * P.n_slots < (1ll << 31), "head rows: more than 2^31 rows");
   if (!some || P.n_slots == 0) return;
-  int lpr = 1;
-  P.lpr_log = 0;
-  while (lpr * 16 < a.head_dim) { lpr *= 2; ++P.lpr_log; }
-  P.per_unit = 1;
-  P.units_per_token = (P.n_slots + P.per_unit - 1) / P.per_unit;
-  P.n_units = (uint32_t)a.tokens * P.units_per_token;
-  P.slots_div = FastDiv::of((uint32_t)P.units_per_token);
+  P.lpr = (uint32_t)a.head_dim / 16;
+  P.lpr_div = FastDiv::of(P.lpr);
+  P.wave_rows = 64 / P.lpr;
+  P.n_rows = (uint32_t)a.tokens * P.n_slots;
+  P.slots_div = FastDiv::of((uint32_t)P.n_slots);
+  P.inv_dim = 1.0f / (float)a.head_dim;
   // 16-byte accesses where every row that the call touches is aligned; else element by element
   const bool vec = rows_aligned(a.q, a.q_token, a.q_head, a.type) && rows_aligned(a.q_out, a.q_out_token, a.q_out_head, a.type) &&
                    rows_aligned(a.k, a.k_token, a.k_head, a.type) && rows_aligned(a.k_out, a.k_out_token, a.k_out_head, a.cache_type) &&

@@ -500,3 +500,22 @@ def test_steps_in_graphs_on_streams_and_at_once(t, ops):
     for group, w in zip(res, want):
         for o in group:
             assert all(t.equal(x, y) for x, y in zip(o, w))
+
+
+@pytest.mark.parametrize("dim", [16, 32, 48, 112, 144, 176, 208, 336, 512])
+def test_norm_rope_of_every_group(t, ops, dim):
+    """Rows of 1 to 32 lanes, a wave's lanes used up or not, more rows than a block; a row of huge, one of tiny values."""
+    g = t.Generator(device="cuda").manual_seed(dim)
+    q = t.randn(67, 5, dim, device="cuda", generator=g)
+    k = t.randn(67, 1, dim, device="cuda", generator=g)
+    q[3, 1] *= 1e12
+    q[4, 2] *= 1e-12
+    w = t.rand(dim, device="cuda", generator=g) + 0.5
+    ang = t.rand(80, 8, device="cuda", generator=g) * 6
+    cos, sin = ang.cos(), ang.sin()
+    pos = t.arange(67, device="cuda", dtype=t.int32)
+    got = ops.qk_norm_rope(q, k, cos, sin, pos, w, None, eps=1e-30)
+    for y, x, wt in zip(got, (q, k), (w, None)):
+        ref, size = norm_rope(wide(x), None if wt is None else wide(wt), wide(cos), wide(sin), wide(pos).astype(int), 1e-30, False)
+        err = np.abs(wide(y) - ref)
+        assert (err <= 32 * 2.0 ** -24 * size + U["f32"] * np.abs(ref)).all(), (err / (size + 1e-300)).max()
