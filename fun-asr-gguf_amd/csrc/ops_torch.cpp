@@ -4,8 +4,10 @@
 // ValueError before anything is enqueued for tensors that do not fit; RuntimeError with the library's message for what it
 // refuses.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -35,12 +37,19 @@ void check(int rc, const char* what) {
 const at::Tensor* tensor(PyObject* o, const char* name) {
   if (o == Py_None) return nullptr;
   NEED(THPVariable_Check(o), c10::str(name, " must be a tensor"));
-  return &THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  NEED(!t.requires_grad() || !c10::GradMode::is_enabled(), c10::str(name, " requires a gradient: call under torch.no_grad()"));
+  NEED(!t.is_neg(), c10::str(name, " is a negated view"));
+  return &t;
 }
 const at::Tensor& gpu(PyObject* o, const char* name) {
   const at::Tensor* t = tensor(o, name);
   NEED(t && t->is_cuda(), c10::str(name, " must be a tensor on the GPU"));
   return *t;
+}
+// a tensor that is written: no two elements in one place
+void written(const at::Tensor& t, const char* name) {
+  NEED(at::has_internal_overlap(t) != at::MemOverlap::Yes, c10::str(name, " has elements that share memory"));
 }
 int type_of(const at::Tensor& t, const char* name) {
   switch (t.scalar_type()) {
@@ -146,6 +155,7 @@ at::Tensor rows_out(const at::Tensor& x, const at::Tensor* out, const char* name
   if (!out) return fresh(x.sizes(), x.scalar_type(), x.device());
   NEED(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type() && out->device() == x.device() && last_contiguous(*out),
        c10::str(name, " must be like its input, with contiguous heads"));
+  written(*out, name);
   return *out;
 }
 
@@ -198,6 +208,8 @@ PyObject* kv_append(PyObject*, PyObject* const* p, Py_ssize_t n) {
   NEED(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && last_contiguous(v), "v must be like k");
   cache_args(kc, vc, k.size(2));
   NEED(kc.size(1) == k.size(1), "the caches must have k's heads");
+  written(kc, "k_cache");
+  written(vc, "v_cache");
   NEED(whole(slots) && vector_of(slots, k.size(0)), "slots must be int32 or int64 [tokens]");
   at::Tensor oq;
   if (q) {
@@ -267,6 +279,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* p, Py_ssize_t n) {
   at::Tensor out;
   if (given) {
     NEED(given->sizes() == q.sizes() && given->scalar_type() == q.scalar_type() && last_contiguous(*given), "out must be like q");
+    written(*given, "out");
     out = *given;
   } else {
     out = fresh(q.sizes(), q.scalar_type(), d);
@@ -328,7 +341,7 @@ PyObject* sample_tokens(PyObject*, PyObject* const* p, Py_ssize_t n) {
   NEED(u.scalar_type() == at::kFloat && vector_of(u, R), "u must be float32 [rows]");
   auto setting = [&](PyObject* o, const char* name, float& one, const float*& each) {
     if (THPVariable_Check(o)) {
-      const at::Tensor& t = THPVariable_Unpack(o);
+      const at::Tensor& t = *tensor(o, name);
       on(d, &t, name);
       NEED(t.scalar_type() == at::kFloat && vector_of(t, R), c10::str(name, " must be a number or float32 [rows]"));
       each = t.data_ptr<float>();
@@ -340,7 +353,7 @@ PyObject* sample_tokens(PyObject*, PyObject* const* p, Py_ssize_t n) {
   setting(p[4], "top_p", a.top_p, a.top_ps);
   setting(p[5], "min_p", a.min_p, a.min_ps);
   if (THPVariable_Check(p[3])) {
-    const at::Tensor& t = THPVariable_Unpack(p[3]);
+    const at::Tensor& t = *tensor(p[3], "top_k");
     on(d, &t, "top_k");
     NEED(t.scalar_type() == at::kInt && vector_of(t, R), "top_k must be a number or int32 [rows]");
     a.top_ks = t.data_ptr<int32_t>();

@@ -5,7 +5,8 @@ cache, attention of a tree of drafted tokens over it, and draws from given rando
 gfx950 kernels on the current stream of their tensors' device, allocate nothing but outputs and workspaces (through torch's
 allocator, on that stream), never synchronise, and can be captured into a graph. A tensor that was made on another stream is
 ordered before the call by its user, as with any torch operation. Wrong shapes, types, strides or devices raise ValueError
-before anything is enqueued; a refusal of the library raises RuntimeError with its message. There is no CPU fallback.
+before anything is enqueued; a refusal of the library raises RuntimeError with its message. There is no CPU fallback and no
+gradient: a tensor that requires one is refused outside torch.no_grad(). Outputs overlap no input, but where it is said.
 
 A program that also creates an Engine imports torch (or this module) before the first one: torch brings a HIP runtime of its
 own, and the engine's library uses it where it is loaded already. The other way round the process holds two, and torch's

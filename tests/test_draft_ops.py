@@ -155,3 +155,14 @@ def test_import_order(first, warned):
     r = subprocess.run([sys.executable, "-W", "always", "-c", prog], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
     assert ("before the first Engine" in r.stderr) == warned
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    x, u = torch.zeros(2, 8, requires_grad=True), torch.zeros(2)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.sample_tokens(x, u)
+    with torch.no_grad(), pytest.raises(ValueError, match="on the GPU"):
+        ops.sample_tokens(x, u)
+    q = torch.zeros(2, 3, 32, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.qk_norm_rope(q, q.detach(), None, None, None)

@@ -519,3 +519,26 @@ def test_norm_rope_of_every_group(t, ops, dim):
         ref, size = norm_rope(wide(x), None if wt is None else wide(wt), wide(cos), wide(sin), wide(pos).astype(int), 1e-30, False)
         err = np.abs(wide(y) - ref)
         assert (err <= 32 * 2.0 ** -24 * size + U["f32"] * np.abs(ref)).all(), (err / (size + 1e-300)).max()
+
+
+def test_outputs_that_share_memory_gradients_and_negated_views_are_refused(t, ops):
+    q = t.randn(4, 2, 32, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        ops.qk_norm_rope(q, q, None, None, None, out_q=t.zeros(1, 2, 32, device="cuda").expand(4, 2, 32))
+    c = t.zeros(1, 2, 8, 32, device="cuda", dtype=t.float16)
+    s = t.arange(4, device="cuda")
+    for kw in [dict(k_cache=c.expand(3, 2, 8, 32), v_cache=c), dict(k_cache=c, v_cache=c[:, :1].expand(1, 2, 8, 32))]:
+        with pytest.raises(ValueError):
+            ops.kv_append(q, q, slots=s, **kw)
+    x, n = t.randn(1, 2, 4, 32, device="cuda", dtype=t.float16), t.zeros(1, device="cuda", dtype=t.int32)
+    kw = dict(k_cache=c, v_cache=c, block_table=n.view(1, 1), context_lens=n)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.tree_attention(x, out=x[:, :1].clone().expand(1, 2, 4, 32), **kw)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.tree_attention(x.clone().requires_grad_(), **kw)
+    with t.no_grad():
+        ops.tree_attention(x.clone().requires_grad_(), **kw)
+    with pytest.raises(ValueError, match="negated"):
+        ops.tree_attention(t._neg_view(x), **kw)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.sample_tokens(t.zeros(2, 8, device="cuda"), t.zeros(2, device="cuda").requires_grad_())
