@@ -19,6 +19,11 @@
 //             such maxima, so only those groups are read again (a few hundred values). Else: the cut within the list by
 //             histograms of its entries, the chunk, the token in it. A row whose cut's bins hold more than CAP values
 //             (thousands of equal logits) is finished by narrowing the cut over the row itself (general_row).
+//
+// Measured (f32, 151936 tokens): one row at top_k 50 k_scan 3.9 us + k_finish 10.3 us, chains of dependent reads and barriers;
+// 61 rows with settings of their own, most top_p 0.95: k_scan 9.5 (3.9 TB/s) + k_hist 21.5 + k_mass 15.8 + k_finish 21 us.
+// k_hist and k_mass keep the vector units 75 % busy with 64-bit exponentials. With 8 / 24 / 32 values a thread for 16 the 61
+// rows take 69 / 74 / 83 us for 68.
 #include "api.h"
 #include "draft_ops.h"
 
@@ -34,7 +39,8 @@ constexpr int KMAX = 1024;  // largest top_k that k_finish makes from the thread
 
 typedef unsigned long long u64;
 
-struct RowState {  // zeroed by k_scan
+struct RowState {  // zeroed by k_scan, which leaves the scales
+  double inv_t, least;       // 1 / temperature; least logit above the maximum (min_p): once a row, not once a thread
   uint32_t arrived, list_n;
   int b_lo, b_hi, b_k;       // bins of the cut: the listed ones are [b_lo, b_hi] and b_k
   u64 mass_lo, mass_k;       // mass before b_lo / before b_k
@@ -63,20 +69,24 @@ struct SampleP {
 enum RowKind { GREEDY, SMALL_K, HIST, PLAIN };
 struct RowSettings {
   float top_p;
-  double inv_t, least;  // 1 / temperature; least logit above the maximum (min_p)
+  float t, min_p;
   int top_k;
   bool has_k, has_p;
   RowKind kind;
 };
 __device__ __forceinline__ RowSettings settings_of(const fa_sample_args& a, int r) {
   RowSettings s;
-  const float t = a.temperatures ? a.temperatures[r] : a.temperature, m = a.min_ps ? a.min_ps[r] : a.min_p;
-  s.top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-  s.top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+  // (read unconditionally, from u where there is no array: four loads side by side, not one after the other)
+  const float t_r = (a.temperatures ? a.temperatures : a.u)[r], m_r = (a.min_ps ? a.min_ps : a.u)[r];
+  const float p_r = (a.top_ps ? a.top_ps : a.u)[r];
+  const int32_t k_r = (a.top_ks ? a.top_ks : reinterpret_cast<const int32_t*>(a.u))[r];
+  const float t = a.temperatures ? t_r : a.temperature, m = a.min_ps ? m_r : a.min_p;
+  s.top_p = a.top_ps ? p_r : a.top_p;
+  s.top_k = a.top_ks ? k_r : a.top_k;
   s.has_k = s.top_k > 0 && s.top_k < a.vocab;
   s.has_p = s.top_p < 1.f;
-  s.inv_t = 1.0 / (double)t;
-  s.least = m > 0.f ? ::log((double)m) : -INFINITY;
+  s.t = t;
+  s.min_p = m;
   s.kind = !(t > 0.f) || s.top_k == 1 || !(s.top_p > 0.f) || !(m <= 1.f) ? GREEDY
            : s.has_k && s.top_k <= KMAX                                    ? SMALL_K
            : s.has_k || s.has_p                                            ? HIST
@@ -99,8 +109,9 @@ __device__ __forceinline__ int bin_of(float x, float top) {
 }
 __device__ __forceinline__ double rel_of(float x, float top) { return x == top ? 0.0 : (double)x - (double)top; }
 // exp(x) 2^S, rounded to an integer, for x <= 0 and S <= 50: x = n ln 2 + 4 r with |r| <= ln 2 / 8, the Taylor polynomial of
-// degree 9 in r (remainder r^10 / 10! < 7e-18 of 1), squared twice: relative error below 4e-15 before the rounding. Adding
-// 1.5 2^52 leaves n, adding 2^52 the result, in the low bits of a sum: no conversions
+// degree 7 in r (remainder r^8 / 8! < 8e-14 of 1), squared twice: relative error below 4e-13 before the rounding, what a sum
+// over a few thousand tokens of equal weight resolves at S = 44. Adding 1.5 2^52 leaves n, adding 2^52 the result, in the low
+// bits of a sum: no conversions
 __device__ __forceinline__ u64 weight(double x, int S) {
   if (!(x > -60.0)) return 0;  // 2^50 exp(-60) < 1/2 (NaN: -inf times 1 / inf)
   const double t = fma(x, 1.4426950408889634, 0x1.8p52);
@@ -108,9 +119,7 @@ __device__ __forceinline__ u64 weight(double x, int S) {
   const double nf = t - 0x1.8p52;
   double r = fma(nf, -0x1.62e42fefa39efp-1, x);
   r = fma(nf, -0x1.abc9e3b39803fp-56, r) * 0.25;
-  double p = 1.0 / 362880.0;
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
+  double p = 1.0 / 5040.0;
   p = fma(p, r, 1.0 / 720.0);
   p = fma(p, r, 1.0 / 120.0);
   p = fma(p, r, 1.0 / 24.0);
@@ -157,7 +166,18 @@ __device__ __forceinline__ int index_at(bool vec, int base, int t, int e) {
 template <typename T, int BT, int N>
 __device__ __forceinline__ void load_chunk(const RowView<T>& v, int base, int t, float (&x)[N]) {
   constexpr int W = kWide<T>;
-  if (v.vec) {
+  if (v.vec && base + BT * N <= v.V) {  // a whole chunk: all loads before the first use
+    uint4 raw[N / W];
+#pragma unroll
+    for (int j = 0; j < N / W; ++j) raw[j] = *reinterpret_cast<const uint4*>(v.p + base + (j * BT + t) * W);
+#pragma unroll
+    for (int j = 0; j < N / W; ++j) {
+      T y[W];
+      *reinterpret_cast<uint4*>(y) = raw[j];
+#pragma unroll
+      for (int w = 0; w < W; ++w) x[j * W + w] = clean((float)y[w]);
+    }
+  } else if (v.vec) {
 #pragma unroll
     for (int j = 0; j < N / W; ++j) {
       const int i = base + (j * BT + t) * W;
@@ -178,6 +198,15 @@ __device__ __forceinline__ void load_chunk(const RowView<T>& v, int base, int t,
       x[e] = i < v.V ? clean((float)v.p[i]) : -INFINITY;
     }
   }
+}
+
+// the row's largest value alone, in two steps: the first 64 chunks' loads go out at once, to be used later
+__device__ __forceinline__ float row_max_begin(const SampleP& P, int r) {
+  return P.cmax[(int64_t)r * P.chunks + min((int)(threadIdx.x & 63), P.chunks - 1)];
+}
+__device__ __forceinline__ float row_max_end(const SampleP& P, int r, float top) {
+  for (int c = 64 + (threadIdx.x & 63); c < P.chunks; c += 64) top = fmaxf(top, P.cmax[(int64_t)r * P.chunks + c]);
+  return wave_max(top);
 }
 
 // 64-bit sums over a wave by data-parallel moves: within rows of 16 lanes by 1, 2, 4, 8, then a row's last lane to the rows
@@ -247,9 +276,10 @@ __device__ __forceinline__ float row_top(const SampleP& P, int r, int& at) {
   at = 0x7FFFFFFF;
   for (int c = lane; c < P.chunks; c += 64) {  // every wave for itself: no barrier
     const float x = P.cmax[(int64_t)r * P.chunks + c];
+    const int j = P.cidx[(int64_t)r * P.chunks + c];
     if (x > top) {
       top = x;
-      at = P.cidx[(int64_t)r * P.chunks + c];
+      at = j;
     }
   }
 #pragma unroll
@@ -377,6 +407,7 @@ __device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, 
   constexpr int BT = ST, NW = BT / 64;
   const fa_sample_args& a = P.a;
   const RowSettings s = settings_of(a, r);
+  const double inv_t = P.state[r].inv_t, least = P.state[r].least;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab;
   const T* const row = row_view<T>(a, r).p;
   auto logit = [&](int i) { return clean((float)row[i]); };
@@ -544,7 +575,7 @@ __device__ __forceinline__ void general_row(Shared& S, const SampleP& P, int r, 
     const float x = logit(i);
     if (x == -INFINITY || !within(order_key(x), i, cut)) return 0;
     const double rel = rel_of(x, top);
-    return rel < s.least ? 0 : weight(rel * s.inv_t, P.S);
+    return rel < least ? 0 : weight(rel * inv_t, P.S);
   };
   const int seg = ((V + NW - 1) / NW + 63) / 64 * 64, i0 = min(V, wave * seg), i1 = min(V, i0 + seg);
   u64 sum = 0;
@@ -628,7 +659,13 @@ __global__ __launch_bounds__(BT) void k_scan(SampleP P) {
       P.hist_mass[(int64_t)r * BINS + i] = 0;
       P.hist_cnt[(int64_t)r * BINS + i] = 0;
     }
-    if (tid == 0) P.state[r] = RowState{};
+    if (tid == 0) {
+      RowState z{};
+      const RowSettings w = settings_of(P.a, r);
+      z.inv_t = 1.0 / (double)w.t;
+      z.least = w.min_p > 0.f ? ::log((double)w.min_p) : -INFINITY;
+      P.state[r] = z;
+    }
   }
 }
 
@@ -636,6 +673,7 @@ __global__ __launch_bounds__(BT) void k_scan(SampleP P) {
 template <typename T, int CT>
 __device__ __forceinline__ void finish_small_k(Shared& S, const SampleP& P, int r, const RowSettings& s, float top) {
   const int tid = threadIdx.x, lane = tid & 63;
+  const double inv_t = P.state[r].inv_t, least = P.state[r].least;
   const RowView<T> v = row_view<T>(P.a, r);
   const float* const tm = P.tmax + (int64_t)r * P.chunks * CT;
   const int groups = P.chunks * CT;
@@ -699,7 +737,7 @@ __device__ __forceinline__ void finish_small_k(Shared& S, const SampleP& P, int 
   if (tid < n) {
     e = S.list[tid];
     const double rel = rel_of(key_value(entry_key(e)), top);
-    w = rel < s.least ? 0 : weight(rel * s.inv_t, P.S);
+    w = rel < least ? 0 : weight(rel * inv_t, P.S);
   }
   __syncthreads();
   if (tid < n) {
@@ -741,18 +779,19 @@ template <typename T>
 __global__ __launch_bounds__(ST, 8) void k_hist(SampleP P) {
   __shared__ HistShared S;
   const int r = (int)P.grid_div.div(blockIdx.x), c = (int)blockIdx.x - r * P.grid_chunks;
-  const RowSettings s = settings_of(P.a, r);
-  if (s.kind != HIST) return;
-  int at;
-  const float top = row_top(P, r, at);
-  if (top == -INFINITY) return;
   const int tid = threadIdx.x;
-  S.cnt[tid] = 0;
-  S.mass[tid] = 0;
-  __syncthreads();
+  // (all loads first; a row that needs no histogram has read its values in vain)
+  const float first = row_max_begin(P, r);
+  const RowSettings s = settings_of(P.a, r);
   const RowView<T> v = row_view<T>(P.a, r);
   float x[PER];
   load_chunk<T, ST, PER>(v, c * PER * ST, tid, x);
+  if (s.kind != HIST) return;
+  const float top = row_max_end(P, r, first);
+  if (top == -INFINITY) return;
+  S.cnt[tid] = 0;
+  S.mass[tid] = 0;
+  __syncthreads();
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     if (x[e] == -INFINITY) continue;
@@ -815,30 +854,40 @@ __global__ __launch_bounds__(ST, 8) void k_hist(SampleP P) {
 template <typename T, int BT>
 __global__ __launch_bounds__(BT) void k_mass(SampleP P) {
   __shared__ u64 part[BT / 64];
+  __shared__ float kept[BT * PER];
   const int r = (int)P.grid_div.div(blockIdx.x), c = (int)blockIdx.x - r * P.grid_chunks;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  RowState* const st = P.state + r;
+  const float first = row_max_begin(P, r);  // (all loads first, as in k_hist)
+  const int cut_lo = st->b_lo, cut_hi = st->b_hi, cut_k = st->b_k;
+  const double inv_t = st->inv_t, least = st->least;
   const RowSettings s = settings_of(P.a, r);
-  if (s.kind != HIST && s.kind != PLAIN) return;
   const RowView<T> v = row_view<T>(P.a, r);
   float x[PER];
   load_chunk<T, BT, PER>(v, c * PER * BT, tid, x);
-  int at;
-  const float top = row_top(P, r, at);
+  if (s.kind != HIST && s.kind != PLAIN) return;
+  const float top = row_max_end(P, r, first);
   if (top == -INFINITY) return;
-  RowState* const st = P.state + r;
   const bool hist = s.kind == HIST;
-  const int b_lo = hist ? st->b_lo : BINS, b_hi = hist ? st->b_hi : -1, b_k = hist ? st->b_k : -1;
+  const int b_lo = hist ? cut_lo : BINS, b_hi = hist ? cut_hi : -1, b_k = hist ? cut_k : -1;
+  // the values inside the cut move together first, as few of a row's are: a wave has 64 x 16 values and takes as many
+  // exponentials as it has rounds of 64 kept ones (61 rows of top_p 0.95: 18.8 us without, 18.3 with; all loads side by
+  // side and the row's scales from its state: 15.8)
   u64 sum = 0;
-  uint32_t listed = 0;
+  uint32_t listed = 0, n = 0;
+  float* const mine = kept + wave * 64 * PER;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    if (x[e] == -INFINITY) continue;
     const int b = bin_of(x[e], top);
-    if (b < b_lo) {
-      const double rel = rel_of(x[e], top);
-      if (!(rel < s.least)) sum += weight(rel * s.inv_t, P.S);
-    }
-    if ((b >= b_lo && b <= b_hi) || b == b_k) listed |= 1u << e;
+    const bool keep = x[e] != -INFINITY && b < b_lo;
+    const u64 who = __ballot(keep);
+    if (keep) mine[n + __popcll(who & ((1ull << lane) - 1))] = x[e];
+    n += (uint32_t)__popcll(who);
+    if (x[e] != -INFINITY && ((b >= b_lo && b <= b_hi) || b == b_k)) listed |= 1u << e;
+  }
+  for (uint32_t i = lane; i < n; i += 64) {
+    const double rel = rel_of(mine[i], top);
+    if (!(rel < least)) sum += weight(rel * inv_t, P.S);
   }
   if (__any(listed != 0)) {  // a place in the row's list for the whole wave's, then for each lane's
     const int own = __popc(listed);
@@ -1010,7 +1059,7 @@ __device__ __forceinline__ void finish_masses(Shared& S, const SampleP& P, int r
     const u64 e = S.list[i];
     if (!within(entry_key(e), (int)(uint32_t)e, cut)) continue;
     const double rel = rel_of(key_value(entry_key(e)), top);
-    if (!(rel < s.least)) atomicAdd(&S.mass[(uint32_t)e / (PER * CT)], weight(rel * s.inv_t, P.S));
+    if (!(rel < st.least)) atomicAdd(&S.mass[(uint32_t)e / (PER * CT)], weight(rel * st.inv_t, P.S));
   }
   __syncthreads();
   // the chunk: the first whose sum passes the target, or past the end the last with any mass
@@ -1046,7 +1095,7 @@ __device__ __forceinline__ void finish_masses(Shared& S, const SampleP& P, int r
     const float x = i0 + e < v.V ? clean((float)v.p[i0 + e]) : -INFINITY;
     if (x > -INFINITY && within(order_key(x), i0 + e, cut)) {
       const double rel = rel_of(x, top);
-      if (!(rel < s.least)) w[e] = weight(rel * s.inv_t, P.S);
+      if (!(rel < st.least)) w[e] = weight(rel * st.inv_t, P.S);
     }
     own += w[e];
   }

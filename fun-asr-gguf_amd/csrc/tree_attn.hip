@@ -19,6 +19,11 @@
 // 32 bytes, then cover all banks evenly.
 // Blocks of the same rows split the keys where the launch would not fill the card; k_tree_merge joins their partial results
 // (unnormalised output, maximum, sum).
+//
+// Measured: 48 sequences of up to 8191 keys, one token each, 32 / 8 heads of 128: 206 us, 5.0 TB/s of K and V; 32 of up to 2032
+// keys, 16 drafted tokens, 16 / 8 heads: 54 + 6 us (blocks of 1024 keys begin and end for a fifth of it); 4 of 32685 keys, 63
+// drafted tokens, 32 / 8 heads (k_many): 201 us, 670 TFLOP/s, the matrix units busy a third of the time, the waves waiting for
+// operands a third; 8 tokens on 212 keys: 10 us, the chain lengths, page, K, products, V, join.
 #include "api.h"
 #include "draft_ops.h"
 
