@@ -35,6 +35,9 @@ constexpr int PER = 16;     // values a thread
 constexpr int BINS = 1024;  // of 1 / 32 below the maximum; the last takes everything 32 and more below
 constexpr int CAP = 4096;   // values that are sorted
 constexpr int ST = 1024;    // threads of k_hist and k_finish
+// threads of k_scan and k_mass (f32, top_p, 1 / 64 / 512 rows of 151936: 43 / 75 / 324 us, with 1024 threads 52 / 83 / 354;
+// top_k 50: 14 / 20 / 83 and 15 / 23 / 86)
+constexpr int SCAN = 256;
 constexpr int KMAX = 1024;  // largest top_k that k_finish makes from the threads' maxima
 
 typedef unsigned long long u64;
@@ -1155,7 +1158,6 @@ __global__ __launch_bounds__(ST) void k_finish(SampleP P) {
 // -------------------------------------------------------------------------------------------------------------------- host
 struct SamplePlan {
   SampleP P;
-  int bt;
   bool hist, mass;
   int64_t bytes;
 };
@@ -1165,16 +1167,13 @@ static SamplePlan sample_plan(const fa_sample_args* ap) {
   SamplePlan t;
   t.P.a = *ap;
   const fa_sample_args& a = t.P.a;
-  FA_REQUIRE(a.rows >= 0 && a.vocab >= 1 && a.vocab <= (1 << 24), "sample_tokens: rows, or vocab outside 1 .. 2^24");
+  FA_REQUIRE(a.rows >= 0 && a.vocab >= 1 && a.vocab <= PER * SCAN * ST, "sample_tokens: rows, or vocab outside 1 .. 2^22");
   FA_REQUIRE(a.type == FA_F32 || a.type == FA_F16 || a.type == FA_BF16, "sample_tokens: type");
   FA_REQUIRE(a.row_stride >= a.vocab || a.rows <= 1, "sample_tokens: rows overlap");
   int lg = 0;
   while ((1 << lg) < a.vocab) ++lg;
   t.P.S = std::min(50, 62 - lg);  // the whole row's sum stays below 2^62
-  // 256 threads a block up to 8192 blocks (and 1024 chunks, a thread of k_finish each), else 1024
-  const int64_t small = (a.vocab + PER * 256 - 1) / (PER * 256);
-  t.bt = a.rows * small <= 8192 && small <= ST ? 256 : 1024;
-  t.P.chunks = (a.vocab + PER * t.bt - 1) / (PER * t.bt);
+  t.P.chunks = (a.vocab + PER * SCAN - 1) / (PER * SCAN);  // at most ST: k_finish has a thread for each
   t.P.hist_chunks = (a.vocab + PER * ST - 1) / (PER * ST);
   FA_REQUIRE((int64_t)a.rows * t.P.chunks < (1ll << 31), "sample_tokens: more than 2^31 chunks");
   // which launches the rows can need (settings of each row live on the device: all)
@@ -1199,12 +1198,12 @@ static SamplePlan sample_plan(const fa_sample_args* ap) {
   t.P.cmass = reinterpret_cast<u64*>(ws + take(nc * 8));
   t.P.cmax = reinterpret_cast<float*>(ws + take(nc * 4));
   t.P.cidx = reinterpret_cast<int*>(ws + take(nc * 4));
-  t.P.tmax = reinterpret_cast<float*>(ws + take(t.P.want_max ? nc * t.bt * 4 : 0));
+  t.P.tmax = reinterpret_cast<float*>(ws + take(t.P.want_max ? nc * SCAN * 4 : 0));
   t.bytes = at;
   return t;
 }
 
-template <typename T, int BT>
+template <typename T>
 static void sample_run(const SamplePlan& t, hipStream_t s) {
   auto go = [&](void (*kernel)(SampleP), int blocks, int threads) {
     SampleP P = t.P;
@@ -1212,10 +1211,10 @@ static void sample_run(const SamplePlan& t, hipStream_t s) {
     P.grid_div = FastDiv::of((uint32_t)blocks);
     launch(kernel, dim3((uint32_t)P.a.rows * (uint32_t)blocks), dim3(threads), 0, s, P);
   };
-  go(k_scan<T, BT>, t.P.chunks, BT);
+  go(k_scan<T, SCAN>, t.P.chunks, SCAN);
   if (t.hist) go(k_hist<T>, t.P.hist_chunks, ST);
-  if (t.mass) go(k_mass<T, BT>, t.P.chunks, BT);
-  go(k_finish<T, BT>, 1, ST);
+  if (t.mass) go(k_mass<T, SCAN>, t.P.chunks, SCAN);
+  go(k_finish<T, SCAN>, 1, ST);
 }
 
 int64_t sample_tokens_bytes(const fa_sample_args* a) { return sample_plan(a).bytes; }
@@ -1227,9 +1226,9 @@ void sample_tokens(const fa_sample_args* ap, hipStream_t s) {
   FA_REQUIRE(a.logits && a.u && a.token_out, "sample_tokens: null tensor");
   FA_REQUIRE(a.workspace && a.workspace_bytes >= t.bytes && aligned16(a.workspace),
              "sample_tokens: workspace too small or not 16-byte aligned");
-  if (a.type == FA_F32) t.bt == 256 ? sample_run<float, 256>(t, s) : sample_run<float, 1024>(t, s);
-  else if (a.type == FA_F16) t.bt == 256 ? sample_run<_Float16, 256>(t, s) : sample_run<_Float16, 1024>(t, s);
-  else t.bt == 256 ? sample_run<__bf16, 256>(t, s) : sample_run<__bf16, 1024>(t, s);
+  if (a.type == FA_F32) sample_run<float>(t, s);
+  else if (a.type == FA_F16) sample_run<_Float16>(t, s);
+  else sample_run<__bf16>(t, s);
 }
 
 }  // namespace fa

@@ -346,19 +346,19 @@ typedef struct fa_tree_attention_args {
   int32_t q_type, cache_type, pages, page_size, table_len, max_context;
   float scale;
 } fa_tree_attention_args;
-/* Bytes of workspace the call needs (0: none); depends on the sizes, types and max_context alone. */
+/* Bytes of workspace the call needs (0: none); depends on the sizes, types, max_context and the current device alone. */
 int fa_tree_attention_workspace(const fa_tree_attention_args* a, int64_t* bytes);
 int fa_tree_attention(const fa_tree_attention_args* a, void* stream);
 
-/* One token for every row of logits [rows, vocab], from a given random number u[row] in [0, 1): the sampler chain
- * top_k -> top_p (min_keep 1, softmax at temperature 1 over the top_k) -> min_p (p >= min_p * max p) -> temperature, then
- * the first token i, in the vocabulary's order, whose cumulative mass exceeds u * total. Equal logits: the lower id ranks
- * higher. temperature <= 0: the largest logit. top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 switch a step off. NaN
- * logits count as -inf; a row with nothing above -inf gives token -1 and probability 0; +inf logits share the whole mass.
- * Sums are exact integers (weights rounded to 2^-44 of the largest at a vocabulary of 2^18), so a result depends on the
- * row alone. Settings: the scalars, or per-row device arrays where not NULL. prob_out (nullable): the token's
- * probability. fa_sampling's chain draws from its own counters; this one is for callers that bring the random numbers
- * (speculative verification, reproducible serving). */
+/* One token for every row of logits [rows, vocab] (vocab at most 2^22), from a given random number u[row] in [0, 1): the
+ * sampler chain top_k -> top_p (min_keep 1, softmax at temperature 1 over the top_k) -> min_p (p >= min_p * max p) ->
+ * temperature, then the first token i, in the vocabulary's order, whose cumulative mass exceeds u * total. Equal logits: the
+ * lower id ranks higher. temperature <= 0: the largest logit. top_k <= 0 or >= vocab, top_p >= 1 and min_p <= 0 switch a
+ * step off; a setting that is NaN gives the largest logit. NaN logits count as -inf; a row with nothing above -inf gives
+ * token -1 and probability 0; +inf logits share the whole mass. Sums are exact integers (weights rounded to 2^-44 of the
+ * largest at a vocabulary of 2^18), so a result depends on the row alone. Settings: the scalars, or per-row device arrays
+ * where not NULL. prob_out (nullable): the token's probability. fa_sampling's chain draws from its own counters; this one is
+ * for callers that bring the random numbers (speculative verification, reproducible serving). */
 typedef struct fa_sample_args {
   const void* logits;
   const float* u;
