@@ -590,7 +590,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // int8 MFMA returning f32: the accumulator starts at 1.5 * 2^23, so every element is the f32 bit pattern of
 // 12582912 + dot (|dot| <= 32 * 128 * 128 < 2^22) and as_float(D) - 12582912 == (float)dot exactly (both operands in
-// [2^23, 2^24): Sterbenz), two elements per v_pk_add_f32 instead of one v_cvt_f32_i32 each
+// [2^23, 2^24): Sterbenz)
 // (MAGIC = false: the plain conversion, for kernels where the constant's 16 registers would spill)
 template <bool MAGIC = true>
 __device__ __forceinline__ f32x16 mfma_i8_f32(const i32x4_t& a, const i32x4_t& b) {
@@ -603,6 +603,24 @@ __device__ __forceinline__ f32x16 mfma_i8_f32(const i32x4_t& a, const i32x4_t& b
     const i32x16_t zero = {};
     return __builtin_convertvector(__builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, zero, 0, 0, 0), f32x16);
   }
+}
+
+// d_w[row] * d_x[token] of one q8_0 block over a 32x32 tile, in the layout of the int8 product: an outer product on the matrix
+// units, which are idle while the vector units convert and accumulate (16 scalar products a block otherwise, the packed forms
+// being off). Lane (r, h) gives d_w of row r and d_x of token r to k slot h: one half of the wave (`own`) the real ones, the other
+// 0 * 0, so every value is the scalar product, rounded once.
+__device__ __forceinline__ f32x16 scale_tile(float dw, float dx, bool own) {
+  const f32x16 zero = {};
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(own ? dw : 0.f, own ? dx : 0.f, zero, 0, 0, 0);
+}
+// acc += f32(dot) * scale: one rounding per fused add
+__device__ __forceinline__ void add_block(f32x16& acc, const i32x4_t& a, const i32x4_t& b, const f32x16& scale) {
+  const i32x16_t zero = {};
+  const f32x16 D = __builtin_convertvector(__builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, zero, 0, 0, 0), f32x16);
+  acc = __builtin_elementwise_fma(D, scale, acc);
+}
+__device__ __forceinline__ float half_of(uint32_t two, int which) {
+  return __half2float(reinterpret_cast<const __half*>(&two)[which]);
 }
 
 // Scales of NBW consecutive q8_0 blocks of one weight row (fp16, NBW/2 dwords): one load instruction
@@ -859,43 +877,15 @@ __device__ __forceinline__ void sk_tile(const GemvArgs& a, int K, int KS, int bx
       B[j] = *reinterpret_cast<const i32x4_t*>(&s_ab[wave][1][r * SLD + 32 * j + 16 * h]);
     }
   }
-  // the wave's weight scales as f32 in LDS, [block][row], in its own staging image past the 4 KB that s_red takes
-  // below (its fragments are in registers by now); lane (r, h) reads rows 8 g + 4 h + [0, 4) of block j as a float4
-  static_assert(16 * 64 * 4 + NBW * 32 * 4 <= 2 * 32 * SLD, "k_gemm_q8_sk: scales must fit the wave's staging image");
-  float4(&s_dw4)[NBW][8] = *reinterpret_cast<float4(*)[NBW][8]>(&s_ab[wave][0][16 * 64 * 4]);
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // fragment reads before the scale writes
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  {
-    float* s_dw = reinterpret_cast<float*>(&s_dw4[0][0]);
+  f32x16 acc2 = {};
 #pragma unroll
-    for (int q = 0; q < SQ; ++q) {
-      const __half* hq = reinterpret_cast<const __half*>(&dwr[q]);
-      const int j = (NBW >= 4 ? 2 * SQ * h : 0) + 2 * q;
-      s_dw[j * 32 + r] = __half2float(hq[0]);
-      s_dw[(j + 1) * 32 + r] = __half2float(hq[1]);
-    }
-  }
-  f32x2_t acc2[8];  // regs 2 p, 2 p + 1
-#pragma unroll
-  for (int p = 0; p < 8; ++p) acc2[p] = f32x2_t{0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < NBW; ++j) {
-    // (the 1.5 * 2^23 accumulator start of mfma_i8_f32 measured 1 % slower here)
-    const i32x16_t D = __builtin_amdgcn_mfma_i32_32x32x32_i8(A[j], B[j], zero, 0, 0, 0);
+  for (int j = 0; j < NBW; ++j) {  // (lane half h holds the scales of blocks [2 SQ h, 2 SQ h + 2 SQ); NBW < 4: both hold all)
     const float dx = (j & 1) ? dx2[j >> 1].y : dx2[j >> 1].x;
-    // acc += f32(dot) * (f32(d_w) * d_x): the scalar form's roundings, two values per instruction
-#pragma unroll
-    for (int gq = 0; gq < 4; ++gq) {
-      const float4 d4 = s_dw4[j][2 * gq + h];
-      const f32x2_t lo = f32x2_t{d4.x, d4.y} * dx, hi = f32x2_t{d4.z, d4.w} * dx;
-      acc2[2 * gq] = __builtin_elementwise_fma(f32x2_t{(float)D[4 * gq], (float)D[4 * gq + 1]}, lo, acc2[2 * gq]);
-      acc2[2 * gq + 1] =
-          __builtin_elementwise_fma(f32x2_t{(float)D[4 * gq + 2], (float)D[4 * gq + 3]}, hi, acc2[2 * gq + 1]);
-    }
+    const bool own = NBW >= 4 ? h == j / (2 * SQ) : h == 0;
+    add_block(acc2, A[j], B[j], scale_tile(half_of(dwr[(j % (2 * SQ)) / 2], j & 1), dx, own));
   }
 #pragma unroll
-  for (int reg = 0; reg < 16; ++reg) acc[reg] = acc2[reg >> 1][reg & 1];
+  for (int reg = 0; reg < 16; ++reg) acc[reg] = acc2[reg];
   // fixed-order reduction over the waves
   // s_red[w] in wave w's own staging image (written after the wave read its fragments, read after the barrier)
   static_assert(16 * 64 * 4 <= 2 * 32 * SLD, "k_gemm_q8_sk: wave partials must fit the wave's staging image");
@@ -1056,7 +1046,6 @@ __global__ __launch_bounds__(256, LMB_PER_CU) void k_lm_head_b(GemvArgs a) {
   const int t_b = min(r, a.M - 1);
   const int n_tiles = (a.O + 31) >> 5;
   __shared__ __attribute__((aligned(16))) int8_t s_w[4][32 * WLD];  // per wave: its K quarter of the tile's 32 rows
-  __shared__ __attribute__((aligned(16))) float s_sc[4][NBW][64];  // per wave: [block j][lane -> row lane & 31], f32
   // s_red[wave] aliases the wave's own weight image: written after the wave has read its A fragments, read between
   // the two barriers, and the image is rewritten only after the second barrier
   static_assert(16 * 64 * 4 <= 32 * WLD, "k_lm_head_b: wave partials must fit the wave's weight image");
@@ -1113,44 +1102,20 @@ __global__ __launch_bounds__(256, LMB_PER_CU) void k_lm_head_b(GemvArgs a) {
 #pragma unroll
     for (int i = 0; i < NBW; ++i)
       *reinterpret_cast<i32x4_t*>(sw + (4 * i + (lane >> 4)) * WLD + 16 * (lane & 15)) = W[i];
-    {  // row r's 8 scales as f32, transposed so a fragment's 16 rows are 4 x 16-B reads (every lane: no branch)
-      const uint32_t pr[4] = {sl.x, sl.y, sl.z, sl.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const __half* hp = reinterpret_cast<const __half*>(&pr[k]);
-        s_sc[wave][2 * k][lane] = __half2float(hp[0]);
-        s_sc[wave][2 * k + 1][lane] = __half2float(hp[1]);
-      }
-    }
+    const uint32_t pr[4] = {sl.x, sl.y, sl.z, sl.w};  // row r's 8 scales
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     if (tile + (int)gridDim.x < n_tiles) load_tile(tile + gridDim.x, W, sl);
-    f32x2_t acc2[8];  // regs 2 p, 2 p + 1
+    f32x16 acc2 = {};
 #pragma unroll
-    for (int p = 0; p < 8; ++p) acc2[p] = f32x2_t{0.f, 0.f};
-#pragma unroll
-    for (int jp = 0; jp < NBW / 2; ++jp) {
-#pragma unroll
-      for (int jj = 0; jj < 2; ++jj) {
-        const int j = 2 * jp + jj;
-        const i32x4_t Aj = *reinterpret_cast<const i32x4_t*>(sw + r * WLD + 32 * j + 16 * h);  // MFMA layout
-        const i32x16_t D = __builtin_amdgcn_mfma_i32_32x32x32_i8(Aj, B[j], zero, 0, 0, 0);
-        // block j's scales of rows (reg & 3) + 8 (reg >> 2) + 4 h (wave-half broadcast reads); acc += f32(dot) *
-        // (d_w * d_x) with the scalar form's roundings, two values per instruction (v_pk_mul_f32 / v_pk_fma_f32)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 v = *reinterpret_cast<const float4*>(&s_sc[wave][j][8 * q + 4 * h]);
-          const f32x2_t lo = f32x2_t{v.x, v.y} * dx[j], hi = f32x2_t{v.z, v.w} * dx[j];
-          acc2[2 * q] = __builtin_elementwise_fma(f32x2_t{(float)D[4 * q], (float)D[4 * q + 1]}, lo, acc2[2 * q]);
-          acc2[2 * q + 1] =
-              __builtin_elementwise_fma(f32x2_t{(float)D[4 * q + 2], (float)D[4 * q + 3]}, hi, acc2[2 * q + 1]);
-        }
-      }
+    for (int j = 0; j < NBW; ++j) {
+      const i32x4_t Aj = *reinterpret_cast<const i32x4_t*>(sw + r * WLD + 32 * j + 16 * h);  // MFMA layout
+      add_block(acc2, Aj, B[j], scale_tile(half_of(pr[j >> 1], j & 1), dx[j], h == 0));
     }
 #pragma unroll
     for (int reg = 0; reg < 16; ++reg)
-      *reinterpret_cast<float*>(s_w[wave] + (reg * 64 + lane) * 4) = acc2[reg >> 1][reg & 1];
+      *reinterpret_cast<float*>(s_w[wave] + (reg * 64 + lane) * 4) = acc2[reg];
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -1428,39 +1393,21 @@ __global__ __launch_bounds__(NW * 64) void k_gemm_q8_kw(GemvArgs a, int K) {
       dx2[q].y = __half2float(__float2half_rn(rstd * dx2[q].y));
     }
   }
-  // the wave's scales as f32 in LDS, [block][row]: each lane then reads its 16 rows' (rows 8 g + 4 h + [0, 4)) of a
-  // block as 4 float4, converted once per wave instead of once per lane (wave-private rows: no block barrier)
-  __shared__ float4 s_dw4[NW][NBW][8];
-  float* s_dw = reinterpret_cast<float*>(s_dw4[wave]);
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    const __half* hq = reinterpret_cast<const __half*>(&dwr[q]);
-    const int j = h * (NBW / 2) + 2 * q;
-    s_dw[j * 32 + r] = __half2float(hq[0]);
-    s_dw[(j + 1) * 32 + r] = __half2float(hq[1]);
-  }
   __builtin_amdgcn_sched_barrier(0);
-  f32x2_t acc[8];  // regs 2 p, 2 p + 1
-#pragma unroll
-  for (int p = 0; p < 8; ++p) acc[p] = f32x2_t{0.f, 0.f};
-  const i32x16_t zero = {};
+  f32x16 acc = {};
 #ifdef FA_GEMV_STAMPS
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   GSTAMP(1);
 #endif
 #pragma unroll
   for (int j = 0; j < NBW; ++j) {
-    const i32x16_t D = __builtin_amdgcn_mfma_i32_32x32x32_i8(A[j], B[j], zero, 0, 0, 0);  // (1.5 * 2^23 start: no gain)
+    // one block at a time: the products depend on nothing else, and hipcc would make them all first and spill them
+    asm volatile("" : "+v"(A[j]));
     const float dx = (j & 1) ? dx2[j >> 1].y : dx2[j >> 1].x;
-    // acc += f32(dot) * (f32(d_w) * d_x): one rounding per product and per fused add, as the scalar form, two
-    // values per instruction (v_pk_mul_f32 / v_pk_fma_f32)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float4 d4 = s_dw4[wave][j][2 * g + h];
-      const f32x2_t lo = f32x2_t{d4.x, d4.y} * dx, hi = f32x2_t{d4.z, d4.w} * dx;
-      acc[2 * g] = __builtin_elementwise_fma(f32x2_t{(float)D[4 * g], (float)D[4 * g + 1]}, lo, acc[2 * g]);
-      acc[2 * g + 1] = __builtin_elementwise_fma(f32x2_t{(float)D[4 * g + 2], (float)D[4 * g + 3]}, hi, acc[2 * g + 1]);
-    }
+    float dw = half_of(dwr[(j % (NBW / 2)) / 2], j & 1);
+    asm volatile("" : "+v"(dw));
+    add_block(acc, A[j], B[j], scale_tile(dw, dx, h == j / (NBW / 2)));
+    asm volatile("" : "+v"(acc));
   }
   // fixed-order reduction over the waves of each matrix (NW = 16: waves w and w + 8 first pair up); thread t then
   // finalises regs [RPT (t>>6), +RPT) of lane t&63
@@ -1472,18 +1419,18 @@ __global__ __launch_bounds__(NW * 64) void k_gemm_q8_kw(GemvArgs a, int K) {
   if (NW == 16) {
     if (wave >= 8) {
 #pragma unroll
-      for (int reg = 0; reg < 16; ++reg) s_red[wave - 8][reg][lane] = acc[reg >> 1][reg & 1];
+      for (int reg = 0; reg < 16; ++reg) s_red[wave - 8][reg][lane] = acc[reg];
     }
     __syncthreads();
     if (wave < 8) {
 #pragma unroll
-      for (int reg = 0; reg < 16; ++reg) acc[reg >> 1][reg & 1] += s_red[wave][reg][lane];
+      for (int reg = 0; reg < 16; ++reg) acc[reg] += s_red[wave][reg][lane];
     }
     __syncthreads();
   }
   if (wave < NR) {
 #pragma unroll
-    for (int reg = 0; reg < 16; ++reg) s_red[wave][reg][lane] = acc[reg >> 1][reg & 1];
+    for (int reg = 0; reg < 16; ++reg) s_red[wave][reg][lane] = acc[reg];
   }
   __syncthreads();
   GSTAMP(2);
@@ -1725,9 +1672,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_q8_t(GemvArgs a, int K) {
 #pragma unroll
           for (int jj = 0; jj < 2; ++jj) {
             const f32x16 D = mfma_i8_f32<EPI != 2>(aw, bx[jj]);  // SwiGLU form: 255 VGPRs already
-            // acc += f32(dot) * (f32(d_w) * d_x), one rounding per product and per fused add as before, on 16-wide
-            // vectors: v_pk_mul_f32 / v_pk_fma_f32 (two values per instruction; hipcc packed the EPI 0 / 1 forms by
-            // itself but not the SwiGLU one)
+            // acc += f32(dot) * (f32(d_w) * d_x), one rounding per product and per fused add
             acc[m][i][jj] = __builtin_elementwise_fma(D, dwv * dx[jj], acc[m][i][jj]);
           }
           __builtin_amdgcn_sched_barrier(0);  // one (matrix, row tile) at a time: two MFMA results live, not eight
