@@ -2080,9 +2080,6 @@ constexpr int APART = ATTN_PART_FLOATS;  // per-split partial: o[GQ][128], m[GQ]
 // owner wave (which takes its values from LDS) possibly AFTER other waves' clamped loads, so a clamped re-read of it
 // would see stale bytes -- bytes a previous buffer left there, possibly NaN / Inf patterns -- and a masked key's
 // p = 0 times a NaN V is NaN. Masked keys re-read row pos - 1 instead (written, finite): valid keys are unchanged.
-#ifndef FA_KV_CLAMP_OLD  // 1 (A/B builds only): the pre-round-6 clamp to row pos (reproduces the stale-row read)
-#define FA_KV_CLAMP_OLD 0
-#endif
 template <int NI, int AW>
 __device__ __forceinline__ void load_kv_groups(const __half* __restrict__ base, int KV, int g0, int kmax, int kq,
                                                int dq, int4 (&t)[NI]) {
@@ -2141,7 +2138,7 @@ __device__ __forceinline__ void attn_wave(const __half* __restrict__ kb, const _
                                           float (&mx)[GQ], float (&l)[GQ], float (&acc)[GQ][8],
                                           const int4* pk = nullptr, const int4* pv = nullptr, int4* slot = nullptr) {
   constexpr int SD = 128;
-  const int kmax = decode && !FA_KV_CLAMP_OLD ? max(pos - 1, 0) : n_keys - 1;  // last cache row a load may touch
+  const int kmax = decode ? max(pos - 1, 0) : n_keys - 1;  // last cache row a load may touch
   auto lpf_issue = [&](int g1) {  // next pass's groups -> slot (clamped rows as load_kv_groups clamps them)
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -3572,8 +3569,8 @@ __device__ __forceinline__ void kv_early(const AttnOArgs& a, int g, int sp, int 
   if (g0 >= ge) return;
   const __half* kb = a.kc + (int64_t)seq * a.seq_stride + g * a.head_stride;
   const __half* vb = a.vc + (int64_t)seq * a.seq_stride + g * a.head_stride;
-  load_kv_groups<AKV_PRE, AWV>(kb, a.KV, g0, FA_KV_CLAMP_OLD ? pos : max(pos - 1, 0), lane >> 4, lane & 15, pk);
-  load_kv_groups<AKV_PRE, AWV>(vb, a.KV, g0, FA_KV_CLAMP_OLD ? pos : max(pos - 1, 0), lane >> 4, lane & 15, pv);
+  load_kv_groups<AKV_PRE, AWV>(kb, a.KV, g0, max(pos - 1, 0), lane >> 4, lane & 15, pk);
+  load_kv_groups<AKV_PRE, AWV>(vb, a.KV, g0, max(pos - 1, 0), lane >> 4, lane & 15, pv);
 }
 
 int g_l2pf_blocks = 16;
