@@ -707,14 +707,15 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeP P) {
   f *= sum == 0.f ? 0.f : 1.f / sum;
   constexpr int N = DP / 64;
   float x[N] = {};
+  // (every lane takes part, also those behind head_dim, whose sums are not stored: their weights are asked for. A partial row
+  // has DP places)
   const float* const o = P.part_o + at0 * DP + lane * N;
-  if (lane * N < a.head_dim)
 #pragma unroll 4
-    for (int s = 0; s < L.splits; ++s) {
-      const float g = __shfl(f, s);
+  for (int s = 0; s < L.splits; ++s) {
+    const float g = __shfl(f, s);
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] += g * o[(int64_t)s * P.rows * DP + i];
-    }
+    for (int i = 0; i < N; ++i) x[i] += g * o[(int64_t)s * P.rows * DP + i];
+  }
   const int nd = (int)P.group_div.div((uint32_t)rr);
   TO* out = reinterpret_cast<TO*>(a.out) + b * a.out_seq + nd * a.out_node +
             (int64_t)(h * P.group + rr - nd * P.group) * a.out_head + lane * N;
