@@ -240,9 +240,9 @@ __device__ __forceinline__ void apply_mask(uint32_t bits, f32x4 (&s)[2]) {
 }
 
 // An infinity or NaN in a drafted key's value must reach the rows that have a weight for it and no others (in the matrix
-// product 0 * inf would reach every row): the loops leave such values out (strip_nonfinite), and where there were any, this
-// adds them at the end, key by key, for the 32-key groups kt, kt + step ... of the drafted keys. wl: 32 x 16 floats of LDS of
-// the wave's own. Rare, and kept out of the loops for their registers' sake.
+// product 0 * inf would reach every row): the loops leave such values out (strip_nonfinite; a committed key's stay, as every row
+// sees it), and where there were any, this adds them at the end, key by key, for the 32-key groups kt, kt + step ... of the
+// drafted keys. wl: 32 x 16 floats of LDS of the wave's own. Rare, and kept out of the loops for their registers' sake.
 template <typename T, int NS, int DP>
 __device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, const SeqLens& L, int kt, int k1, int step,
                                               int node, const typename Vec8<T>::type (&q)[DP / 32][NS], float m, float* wl,
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           if (gone) vr[t][ks] = V8{};  // whatever lies there must not meet a weight of 0
-          if (drafted) bad |= strip_nonfinite<T>(vr[t][ks]);
+          if (kt + 16 * t + r16 >= L.ctx) bad |= strip_nonfinite<T>(vr[t][ks]);
         }
       }
 #pragma unroll
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         if (!((present >> (i * KPS + row)) & 1)) vr[i] = V8{};
-        if (drafted) bad |= strip_nonfinite<T>(vr[i]);
+        if (kt + i * KPS + row >= L.ctx) bad |= strip_nonfinite<T>(vr[i]);
       }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)

@@ -1,10 +1,10 @@
-"""The drafted-token operators (fun_asr_gguf.ops) on the GPU where they can go wrong: many splits of narrow heads.
-Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
+"""The drafted-token operators (fun_asr_gguf.ops) on the GPU where they can go wrong: many splits of narrow heads,
+infinities and NaN among committed keys. Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
 import numpy as np
 import pytest
 import torch  # noqa: F401  (before any engine: the library then shares torch's HIP runtime)
 
-from test_gpu_draft_ops import check, kind, ops, paged, t  # noqa: F401
+from test_gpu_draft_ops import check, kind, ops, paged, t, trees  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +20,30 @@ def test_attention_splits_of_every_head_size(t, ops, ctx, N, H, KV, D, qn, cn, o
     kc, vc, table = paged(t, ctx, N, 16, KV, D, cn, order, 5)
     q = (2 * t.randn(len(ctx), N, H, D, generator=t.Generator().manual_seed(6))).to(kind(t, qn)).cuda()
     check(t, ops, q, kc, vc, table, ctx, names=(qn, cn))
+
+
+# ---------------------------------------------------------------------------------------- infinities and NaN, committed
+@pytest.mark.parametrize("N", [1, 9, 40])
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [128, 96])
+def test_attention_nonfinite_committed_values_reach_every_row(t, ops, name, N, D):
+    """Wherever the key lies: tiles before the last, the tile that also holds the drafts, the last committed token."""
+    ctx = [100]
+    kc, vc, table = paged(t, ctx, N, 16, 2, D, name, "hpd", 8)
+    q = t.randn(1, N, 4, D, generator=t.Generator().manual_seed(1)).to(kind(t, name)).cuda()
+    mask = trees(t, 1, N, 9) if N > 1 else None
+    lens = t.tensor(ctx, dtype=t.int32).cuda()
+    run = lambda: ops.tree_attention(q, kc, vc, table, lens, mask=None if mask is None else mask.cuda())  # noqa: E731
+    clean = check(t, ops, q, kc, vc, table, ctx, mask, names=(name, name))
+    for p in (10, 63, 64, 95, 96, 99):
+        at = int(table[0, p // 16]), slice(None), p % 16
+        for what in (float("inf"), float("-inf"), float("nan")):
+            for d in (3, 77):
+                keep = vc[at].clone()
+                vc[at[0], :, at[2], d] = what
+                out = run()
+                vc[at] = keep
+                hit = out[..., d]
+                assert (hit.isnan().all() if what != what else (hit == what).all()), (p, what, d)
+                rest = [x for x in range(D) if x != d]
+                assert t.equal(out[..., rest], clean[..., rest]), (p, what, d)
