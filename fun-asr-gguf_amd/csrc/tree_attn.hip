@@ -18,7 +18,7 @@
 // In LDS, row k's 16-byte piece j lies at j ^ (k mod pieces): an operand read's 16 rows, and a transposing read's 16 rows of
 // 32 bytes, then cover all banks evenly.
 // Blocks of the same rows split the keys where the launch would not fill the card; k_tree_merge joins their partial results
-// (unnormalised output, maximum, sum).
+// (unnormalised output, base, sum).
 //
 // Measured: 48 sequences of up to 8191 keys, one token each, 32 / 8 heads of 128: 206 us, 5.0 TB/s of K and V; 32 of up to 2032
 // keys, 16 drafted tokens, 16 / 8 heads: 54 + 6 us (blocks of 1024 keys begin and end for a fifth of it); 4 of 32685 keys, 63
@@ -44,7 +44,7 @@ struct TreeP {
   int n_groups;        // (sequence, kv head, split) triples
   float c;             // scale * log2(e)
   float* part_o;       // [seqs][kv_heads][splits][rows][DP]
-  float* part_ml;      // [seqs][kv_heads][splits][rows][2]
+  float* part_ml;      // [seqs][kv_heads][splits][rows][2]: base (see base_of; -inf: nothing seen) and sum
   int q_vec;           // q's rows may be read in 16-byte pieces
   uint32_t k_page, k_slot, v_page, v_slot;  // strides, below 2^31 (checked by the host): one multiply-add a product
   int one_offset;      // K's and V's strides are the same
@@ -71,6 +71,14 @@ __device__ __forceinline__ float across_sum(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
 }
+// Softmax weights are 2^(s c - base) with base = maximum c - kLift: 2^kLift at the largest. They enter the second product in the
+// cache's type, and so float16's range lies where they do: steps of 2^-11 of a weight down to 2^-29 of the largest, then of
+// 2^-39, nothing under 2^-40 (from 1 down it ends at 2^-25: of 40 000 keys e^-18 under one large weight nothing was left).
+// bfloat16 has the range of float32. The factor leaves with the division by the sum.
+template <typename T> constexpr float kLift = 0.f;
+template <> constexpr float kLift<_Float16> = 15.f;
+template <typename T>
+__device__ __forceinline__ float base_of(float m, float c) { return fmaf(m, c, -kLift<T>); }
 template <typename T> constexpr uint32_t kExp = 0;  // exponent bits
 template <> constexpr uint32_t kExp<_Float16> = 0x7C00u;
 template <> constexpr uint32_t kExp<__bf16> = 0x7F80u;
@@ -170,7 +178,7 @@ __device__ __forceinline__ uint32_t seen_bits(const TreeP& P, int b, int ctx, in
 }
 
 // KG groups of 32 keys of the softmax: scores s -> weights in their place, relative to the running maximum; o and l rescaled
-template <int MT, int KG>
+template <typename T, int MT, int KG>
 __device__ __forceinline__ void softmax_step(f32x4 (&s)[KG][2], float c, float& m, float& l, f32x4 (&o)[MT]) {
   float top = m;
 #pragma unroll
@@ -178,9 +186,9 @@ __device__ __forceinline__ void softmax_step(f32x4 (&s)[KG][2], float c, float& 
 #pragma unroll
     for (int t = 0; t < 2; ++t) top = fmaxf(top, fmaxf(fmaxf(s[g][t][0], s[g][t][1]), fmaxf(s[g][t][2], s[g][t][3])));
   top = across_max(top);
-  const float base = (top == -INFINITY ? 0.f : top) * c;  // nothing seen so far: every weight is 2^-inf = 0
-  if (__any(top != m)) {                                  // (first tiles mostly)
-    const float alpha = exp2_fast(m * c - base);
+  const float base = top == -INFINITY ? 0.f : base_of<T>(top, c);  // nothing seen so far: every weight is 2^-inf = 0
+  if (__any(top != m)) {                                           // (first tiles mostly)
+    const float alpha = m == -INFINITY ? 0.f : exp2_fast(base_of<T>(m, c) - base);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) o[mt] *= alpha;
     l *= alpha;
@@ -253,7 +261,7 @@ __device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, co
   const T* const kbase = reinterpret_cast<const T*>(a.k_cache) + w.h * a.k_head;
   const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + w.h * a.v_head;
   const int32_t* const table = a.block_table + w.b * a.table_seq;
-  const float base = (m == -INFINITY ? 0.f : m) * P.c;
+  const float base = m == -INFINITY ? 0.f : base_of<T>(m, P.c);
   for (; kt < k1; kt += step) {
     if (kt + 32 <= L.ctx) continue;
     f32x4 s[2];
@@ -320,10 +328,10 @@ __device__ __forceinline__ void store4(TO* p, f32x4 x, int left) {
     if (i < left) p[i] = (TO)x[i];
 }
 
-// T: cache type. NS: 16-bit terms of q and of the probabilities (1: q is of the cache's type; 2 / 3: q is float32, kept to 22 /
-// 24 bits by terms of float16 / bfloat16; with 1 term the weights are rounded to the cache's type, half a step of it, as the
-// output is). DP: head_dim rounded up to 64 / 128 / 256. FULL: it is DP itself; else a piece behind head_dim is read at 0
-// instead (q is 0 there, and the output's dimensions behind it are not written).
+// T: cache type. NS: 16-bit terms of q and of the weights (1: q is of the cache's type; 2 / 3: q is float32, kept to 22 / 24
+// bits by terms of float16 / bfloat16, a weight too, float16's down to 2^-40 of the largest; with 1 term the weights are rounded
+// to the cache's type, half a step of it, as the output is). DP: head_dim rounded up to 64 / 128 / 256. FULL: it is DP itself;
+// else a piece behind head_dim is read at 0 instead (q is 0 there, and the output's dimensions behind it are not written).
 // UNI: 16 consecutive keys from a multiple of 16 on lie in one page (page_size is a multiple of 16), so a page's address is a
 // scalar and a lane's place under it a constant 32-bit offset; else every lane looks up its own keys' pages.
 template <typename T, int NS, int DP, int RT, bool FULL, bool UNI>
@@ -445,7 +453,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
     V8 p[RT][NS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      softmax_step<MT, 1>(s[rt], P.c, m[rt], l[rt], o[rt]);
+      softmax_step<T, MT, 1>(s[rt], P.c, m[rt], l[rt], o[rt]);
       to_terms<T, NS>(s[rt][0], p[rt]);
     }
 #pragma unroll
@@ -475,7 +483,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
     const int row = 16 * rt + r16;
     const float sum = across_sum(l[rt]);
     if (g4 == 0) {
-      lml[(wave * ROWS + row) * 2] = m[rt];
+      lml[(wave * ROWS + row) * 2] = m[rt] == -INFINITY ? -INFINITY : base_of<T>(m[rt], P.c);
       lml[(wave * ROWS + row) * 2 + 1] = sum;
     }
 #pragma unroll
@@ -489,12 +497,12 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
     float top = -INFINITY;
 #pragma unroll
     for (int v = 0; v < 4; ++v) top = fmaxf(top, lml[(v * ROWS + row) * 2]);
-    const float base = (top == -INFINITY ? 0.f : top) * P.c;
+    const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      const float f = exp2_fast(lml[(v * ROWS + row) * 2] * P.c - base);
+      const float f = exp2_fast(lml[(v * ROWS + row) * 2] - base);
       sum += f * lml[(v * ROWS + row) * 2 + 1];
       x += f * *reinterpret_cast<const f32x4*>(lo + (v * ROWS + row) * OS + e);
     }
@@ -644,7 +652,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
       if (masked)
 #pragma unroll
         for (int g = 0; g < KG; ++g) apply_mask(bits[rt][g], s[rt][g]);
-      softmax_step<MT, KG>(s[rt], P.c, m[rt], l[rt], o[rt]);
+      softmax_step<T, MT, KG>(s[rt], P.c, m[rt], l[rt], o[rt]);
     }
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
@@ -679,7 +687,9 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
         if (16 * mt + 4 * g4 < D) *reinterpret_cast<f32x4*>(P.part_o + at * DP + 16 * mt + 4 * g4) = o[rt][mt];
-      if (g4 == 0) *reinterpret_cast<float2*>(P.part_ml + at * 2) = make_float2(m[rt], sum);
+      if (g4 == 0)
+        *reinterpret_cast<float2*>(P.part_ml + at * 2) =
+            make_float2(m[rt] == -INFINITY ? -INFINITY : base_of<T>(m[rt], P.c), sum);
     } else {
       typedef typename std::conditional<(NS > 1), float, T>::type TO;
       TO* const out = reinterpret_cast<TO*>(a.out) + w.b * a.out_seq + node[rt] * a.out_node +
@@ -701,8 +711,8 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeP P) {
   const int64_t at0 = ((int64_t)b * a.kv_heads + h) * P.splits * P.rows + rr;
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < L.splits) ml = *reinterpret_cast<const float2*>(P.part_ml + (at0 + (int64_t)lane * P.rows) * 2);
-  const float top = wave_max(ml.x), base = (top == -INFINITY ? 0.f : top) * P.c;
-  float f = exp2_fast(ml.x * P.c - base);
+  const float top = wave_max(ml.x), base = top == -INFINITY ? 0.f : top;
+  float f = exp2_fast(ml.x - base);
   const float sum = wave_sum(f * ml.y);
   f *= sum == 0.f ? 0.f : 1.f / sum;
   constexpr int N = DP / 64;

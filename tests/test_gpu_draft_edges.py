@@ -1,10 +1,11 @@
 """The drafted-token operators (fun_asr_gguf.ops) on the GPU where they can go wrong: many splits of narrow heads,
-infinities and NaN among committed keys. Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
+infinities and NaN among committed keys, weights far below the largest. Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
 import numpy as np
 import pytest
 import torch  # noqa: F401  (before any engine: the library then shares torch's HIP runtime)
 
-from test_gpu_draft_ops import check, kind, ops, paged, t, trees  # noqa: F401
+from draft_oracle import attention
+from test_gpu_draft_ops import check, close, kind, ops, paged, t, tolerance, trees, wide  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,34 @@ def test_attention_nonfinite_committed_values_reach_every_row(t, ops, name, N, D
                 assert (hit.isnan().all() if what != what else (hit == what).all()), (p, what, d)
                 rest = [x for x in range(D) if x != d]
                 assert t.equal(out[..., rest], clean[..., rest]), (p, what, d)
+
+
+# --------------------------------------------------------------------------------------------- weights far below the largest
+@pytest.mark.parametrize("keys,N,gap", [(8192, 1, 18.0), (40000, 1, 17.0), (40000, 1, 18.0), (8192, 40, 18.0), (3000, 2, 21.0)])
+@pytest.mark.parametrize("qn,cn", [("f16", "f16"), ("f32", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+def test_attention_long_tails_below_one_large_weight(t, ops, keys, N, gap, qn, cn):
+    """One key takes nearly all the weight and has a value of 0; the rest, e^-gap below it, make the output. Beside the
+    tolerance of every test: over a float16 cache a weight is a float16 number (two, for a float32 query) of 2^15 at the largest,
+    so its absolute step counts too: half of 2^-24, 2^-40 of the largest weight, for every key."""
+    D = 64
+    g = t.Generator().manual_seed(keys + N)
+    ctx = [keys - N]
+    pages = -(-keys // 64)
+    kc = t.zeros(pages, 1, 64, D)
+    vc = (1 + 0.25 * t.randn(pages, 1, 64, D, generator=g)).abs()
+    kc[..., 0] = 4 + 0.02 * t.randn(pages, 1, 64, generator=g)
+    one = keys // 3
+    kc[one // 64, 0, one % 64, 0] = 4 + gap / 4
+    vc[one // 64, 0, one % 64] = 0
+    kc, vc = (c.to(kind(t, cn)).cuda() for c in (kc, vc))
+    q = t.zeros(1, N, 2, D)
+    q[..., 0] = 4
+    q = q.to(kind(t, qn)).cuda()
+    table = t.arange(pages, dtype=t.int32)[None].cuda()
+    out = ops.tree_attention(q, kc, vc, table, t.tensor(ctx, dtype=t.int32).cuda(), scale=1.0)
+    want, mass, reach = attention(wide(q), wide(kc), wide(vc), table.cpu().numpy(), ctx, [N], None, 1.0)
+    assert want.max() < keys * np.exp(2 - gap)
+    tol = tolerance(want, mass, reach, qn, cn, D)
+    if cn == "f16":
+        tol = tol + keys * 2.0 ** -40 * float(vc.max())
+    close(out, want, tol)
