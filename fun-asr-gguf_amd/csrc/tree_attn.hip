@@ -188,7 +188,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&s)[KG][2], float c, float& 
   top = across_max(top);
   const float base = top == -INFINITY ? 0.f : base_of<T>(top, c);  // nothing seen so far: every weight is 2^-inf = 0
   if (__any(top != m)) {                                           // (first tiles mostly)
-    const float alpha = m == -INFINITY ? 0.f : exp2_fast(base_of<T>(m, c) - base);
+    const float alpha = exp2_fast(base_of<T>(m, c) - base);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) o[mt] *= alpha;
     l *= alpha;
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
     const int row = 16 * rt + r16;
     const float sum = across_sum(l[rt]);
     if (g4 == 0) {
-      lml[(wave * ROWS + row) * 2] = m[rt] == -INFINITY ? -INFINITY : base_of<T>(m[rt], P.c);
+      lml[(wave * ROWS + row) * 2] = base_of<T>(m[rt], P.c);
       lml[(wave * ROWS + row) * 2 + 1] = sum;
     }
 #pragma unroll
@@ -687,9 +687,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
         if (16 * mt + 4 * g4 < D) *reinterpret_cast<f32x4*>(P.part_o + at * DP + 16 * mt + 4 * g4) = o[rt][mt];
-      if (g4 == 0)
-        *reinterpret_cast<float2*>(P.part_ml + at * 2) =
-            make_float2(m[rt] == -INFINITY ? -INFINITY : base_of<T>(m[rt], P.c), sum);
+      if (g4 == 0) *reinterpret_cast<float2*>(P.part_ml + at * 2) = make_float2(base_of<T>(m[rt], P.c), sum);
     } else {
       typedef typename std::conditional<(NS > 1), float, T>::type TO;
       TO* const out = reinterpret_cast<TO*>(a.out) + w.b * a.out_seq + node[rt] * a.out_node +
