@@ -8,6 +8,7 @@ namespace fa {
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));  // (float4 is a struct: four loads, which hipcc need not join again)
 template <typename T> struct Vec8;
 template <> struct Vec8<_Float16> { typedef f16x8_t type; };
 template <> struct Vec8<__bf16> { typedef bf16x8_t type; };
@@ -19,9 +20,12 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
   } else if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = a[i];
+      x[4 + i] = b[i];
+    }
   } else {
     const auto v = *reinterpret_cast<const typename Vec8<T>::type*>(p);
 #pragma unroll

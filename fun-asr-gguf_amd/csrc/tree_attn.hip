@@ -115,35 +115,59 @@ __device__ __forceinline__ bool locate(const TreeP& P, Where& w) {
   return true;
 }
 
-// this lane's query row (of rows r0 + r16) as NS terms of the cache's type: dimensions 8 (g4 + 4 ks) + 0 .. 7
+// this lane's query row (of rows r0 + r16) as NS terms of the cache's type: dimensions 8 (g4 + 4 ks) + 0 .. 7. A float32 row is
+// first multiplied by the power of two that brings its largest element to 2^14 .. 2^15, whatever its size: within float16's range,
+// and with the lower term's steps, 2^-24, 2^-38 of the row's largest. c: what makes scores exponents of 2, with the inverse of it
 template <typename T, int NS, int KS>
 __device__ __forceinline__ int load_q(const TreeP& P, const Where& w, int rr, int rows, int g4,
-                                      typename Vec8<T>::type (&q)[KS][NS]) {
+                                      typename Vec8<T>::type (&q)[KS][NS], float& c) {
   const fa_tree_attention_args& a = P.a;
   const int rc = min(rr, rows - 1), node = (int)P.group_div.div((uint32_t)rc);
   const int64_t at = w.b * a.q_seq + node * a.q_node + (int64_t)(w.h * P.group + rc - node * P.group) * a.q_head;
+  c = P.c;
+  if constexpr (NS == 1) {
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    const int e = 8 * (g4 + 4 * ks);
-    float x[8] = {};
-    if (rr < rows && e < a.head_dim) {
-      if constexpr (NS > 1) {
-        const float* p = reinterpret_cast<const float*>(a.q) + at + e;
-        if (P.q_vec) load8<true>(p, x);
-        else load8<false>(p, x);
-      } else {
-        const T* p = reinterpret_cast<const T*>(a.q) + at + e;
+    for (int ks = 0; ks < KS; ++ks) {
+      const int e = 8 * (g4 + 4 * ks);
+      float x[8] = {};
+      if (rr < rows && e < a.head_dim) {
+        const T* const p = reinterpret_cast<const T*>(a.q) + at + e;
         if (P.q_vec) load8<true>(p, x);
         else load8<false>(p, x);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[ks][0][i] = (T)x[i];
+    }
+  } else {
+    float x[KS][8] = {}, top = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int e = 8 * (g4 + 4 * ks);
+      if (rr < rows && e < a.head_dim) {
+        const float* const p = reinterpret_cast<const float*>(a.q) + at + e;
+        if (P.q_vec) load8<true>(p, x[ks]);
+        else load8<false>(p, x[ks]);
+      }
     }
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[ks][i]));
+    top = across_max(top);  // (an infinite row: the finite elements stay below 2^14)
+    const int f = min(max(268 - (int)(__float_as_uint(top) >> 23), 1), 253);  // exponents of the factor and its inverse
+    const float up = __uint_as_float((uint32_t)f << 23);
+    c = fminf(fmaxf(P.c * __uint_as_float((uint32_t)(254 - f) << 23), 1.2e-38f), 3.4e38f);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const T y = (T)x[i];
-        q[ks][s][i] = y;
-        x[i] -= (float)y;
+        float y = x[ks][i] * up;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const T z = (T)y;
+          q[ks][s][i] = z;
+          y = fabsf(y) < INFINITY ? y - (float)z : 0.f;
+        }
       }
   }
   return node;
@@ -253,7 +277,7 @@ __device__ __forceinline__ void apply_mask(uint32_t bits, f32x4 (&s)[2]) {
 // drafted keys. wl: 32 x 16 floats of LDS of the wave's own. Rare, and kept out of the loops for their registers' sake.
 template <typename T, int NS, int DP>
 __device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, const SeqLens& L, int kt, int k1, int step,
-                                              int node, const typename Vec8<T>::type (&q)[DP / 32][NS], float m, float* wl,
+                                              int node, const typename Vec8<T>::type (&q)[DP / 32][NS], float c, float m, float* wl,
                                               f32x4 (&o)[DP / 16]) {
   typedef typename Vec8<T>::type V8;
   const fa_tree_attention_args& a = P.a;
@@ -261,7 +285,7 @@ __device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, co
   const T* const kbase = reinterpret_cast<const T*>(a.k_cache) + w.h * a.k_head;
   const T* const vbase = reinterpret_cast<const T*>(a.v_cache) + w.h * a.v_head;
   const int32_t* const table = a.block_table + w.b * a.table_seq;
-  const float base = m == -INFINITY ? 0.f : base_of<T>(m, P.c);
+  const float base = m == -INFINITY ? 0.f : base_of<T>(m, c);
   for (; kt < k1; kt += step) {
     if (kt + 32 <= L.ctx) continue;
     f32x4 s[2];
@@ -286,7 +310,7 @@ __device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, co
     apply_mask(seen_bits(P, w.b, L.ctx, kt, present, node, g4), s);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      wl[(16 * (i >> 2) + 4 * g4 + (i & 3)) * 16 + r16] = exp2_fast(fmaf(s[i >> 2][i & 3], P.c, -base));
+      wl[(16 * (i >> 2) + 4 * g4 + (i & 3)) * 16 + r16] = exp2_fast(fmaf(s[i >> 2][i & 3], c, -base));
     for (int k = 0; k < 32 && kt + k < k1; ++k) {
       if (kt + k < L.ctx) continue;
       const uint32_t pg = P.page_div.div((uint32_t)(kt + k));
@@ -400,9 +424,10 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 
   int node[RT];
   V8 q[RT][KS][NS];
+  float c[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) node[rt] = load_q<T, NS, KS>(P, w, r0 + 16 * rt + r16, rows, g4, q[rt]);
-  float m[RT], l[RT];
+  for (int rt = 0; rt < RT; ++rt) node[rt] = load_q<T, NS, KS>(P, w, r0 + 16 * rt + r16, rows, g4, q[rt], c[rt]);
+  float m[RT], l[RT];  // maximum of the scores as the products give them (c[] not applied), sum of the weights
   f32x4 o[RT][MT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -453,7 +478,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
     V8 p[RT][NS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      softmax_step<T, MT, 1>(s[rt], P.c, m[rt], l[rt], o[rt]);
+      softmax_step<T, MT, 1>(s[rt], c[rt], m[rt], l[rt], o[rt]);
       to_terms<T, NS>(s[rt][0], p[rt]);
     }
 #pragma unroll
@@ -472,7 +497,8 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
   if (__any(bad))
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
-      add_nonfinite<T, NS, DP>(P, w, L, k0 + 32 * wave, k1, 128, node[rt], q[rt], m[rt], reinterpret_cast<float*>(vl), o[rt]);
+      add_nonfinite<T, NS, DP>(P, w, L, k0 + 32 * wave, k1, 128, node[rt], q[rt], c[rt], m[rt], reinterpret_cast<float*>(vl),
+                               o[rt]);
 
   // the four waves' results join through LDS
   float* const lo = reinterpret_cast<float*>(smem);  // [4][ROWS][OS]
@@ -483,7 +509,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
     const int row = 16 * rt + r16;
     const float sum = across_sum(l[rt]);
     if (g4 == 0) {
-      lml[(wave * ROWS + row) * 2] = base_of<T>(m[rt], P.c);
+      lml[(wave * ROWS + row) * 2] = base_of<T>(m[rt], c[rt]);
       lml[(wave * ROWS + row) * 2 + 1] = sum;
     }
 #pragma unroll
@@ -581,9 +607,11 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 
   int node[RT];
   V8 q[RT][KS][NS];
+  float c[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) node[rt] = load_q<T, NS, KS>(P, w, r0 + (wave * RT + rt) * 16 + r16, rows, g4, q[rt]);
-  float m[RT], l[RT];
+  for (int rt = 0; rt < RT; ++rt)
+    node[rt] = load_q<T, NS, KS>(P, w, r0 + (wave * RT + rt) * 16 + r16, rows, g4, q[rt], c[rt]);
+  float m[RT], l[RT];  // maximum of the scores as the products give them (c[] not applied), sum of the weights
   f32x4 o[RT][MT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -652,7 +680,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
       if (masked)
 #pragma unroll
         for (int g = 0; g < KG; ++g) apply_mask(bits[rt][g], s[rt][g]);
-      softmax_step<T, MT, KG>(s[rt], P.c, m[rt], l[rt], o[rt]);
+      softmax_step<T, MT, KG>(s[rt], c[rt], m[rt], l[rt], o[rt]);
     }
 #pragma unroll
     for (int g = 0; g < KG; ++g) {
@@ -676,7 +704,8 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
   if (__syncthreads_or(bad))
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
-      add_nonfinite<T, NS, DP>(P, w, L, k0, k1, 32, node[rt], q[rt], m[rt], reinterpret_cast<float*>(smem) + wave * 512, o[rt]);
+      add_nonfinite<T, NS, DP>(P, w, L, k0, k1, 32, node[rt], q[rt], c[rt], m[rt],
+                               reinterpret_cast<float*>(smem) + wave * 512, o[rt]);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int rr = r0 + (wave * RT + rt) * 16 + r16;
@@ -687,7 +716,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
         if (16 * mt + 4 * g4 < D) *reinterpret_cast<f32x4*>(P.part_o + at * DP + 16 * mt + 4 * g4) = o[rt][mt];
-      if (g4 == 0) *reinterpret_cast<float2*>(P.part_ml + at * 2) = make_float2(base_of<T>(m[rt], P.c), sum);
+      if (g4 == 0) *reinterpret_cast<float2*>(P.part_ml + at * 2) = make_float2(base_of<T>(m[rt], c[rt]), sum);
     } else {
       typedef typename std::conditional<(NS > 1), float, T>::type TO;
       TO* const out = reinterpret_cast<TO*>(a.out) + w.b * a.out_seq + node[rt] * a.out_node +

@@ -1,5 +1,5 @@
-"""The drafted-token operators (fun_asr_gguf.ops) on the GPU where they can go wrong: many splits of narrow heads,
-infinities and NaN among committed keys, weights far below the largest. Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
+"""The drafted-token operators (fun_asr_gguf.ops) on the GPU where they can go wrong: many splits of narrow heads, infinities and
+NaN among committed keys, weights far below the largest, float32 queries of any size. Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
 import numpy as np
 import pytest
 import torch  # noqa: F401  (before any engine: the library then shares torch's HIP runtime)
@@ -79,3 +79,37 @@ def test_attention_long_tails_below_one_large_weight(t, ops, keys, N, gap, qn, c
     if cn == "f16":
         tol = tol + keys * 2.0 ** -40 * float(vc.max())
     close(out, want, tol)
+
+
+@pytest.mark.parametrize("size,scale", [(1e5, 1e-6), (1e-4, 1e3), (1e30, 1e-31), (1e-30, 1e28), (None, 0.05)])
+@pytest.mark.parametrize("D,N,cn", [(128, 3, "f16"), (64, 40, "f16"), (96, 2, "bf16"), (256, 20, "f16")])
+def test_attention_float32_queries_of_any_size(t, ops, size, scale, D, N, cn):
+    """Queries past float16's range, or under its steps, at scales that give ordinary scores. None: rows of many sizes in one
+    call, and a row of zeros."""
+    ctx = [130, 3]
+    kc, vc, table = paged(t, ctx, N, 16, 2, D, cn, "hpd", 12)
+    g = t.Generator().manual_seed(3)
+    q = t.randn(2, N, 4, D, generator=g)
+    if size is None:
+        q *= 10 ** (4 * t.rand(2, N, 4, 1, generator=g) - 2)
+        q[0, 0, 1] = 0
+        q[1, 1, :, 1:] = 0
+    else:
+        q *= size
+    check(t, ops, q.cuda(), kc, vc, table, ctx, names=("f32", cn), scale=scale)
+
+
+def test_attention_infinite_float32_queries(t, ops):
+    """An infinite query makes its own row NaN (a score of +inf somewhere) and leaves the others as they are."""
+    ctx, N, D = [50], 4, 128
+    kc, vc, table = paged(t, ctx, N, 16, 2, D, "f16", "hpd", 13)
+    q = t.randn(1, N, 4, D, generator=t.Generator().manual_seed(4)).cuda()
+    lens = t.tensor(ctx, dtype=t.int32).cuda()
+    clean = ops.tree_attention(q, kc, vc, table, lens)
+    for what in (float("inf"), float("-inf"), float("nan")):
+        bad = q.clone()
+        bad[0, 2, 1, 7] = what
+        out = ops.tree_attention(bad, kc, vc, table, lens)
+        assert out[0, 2, 1].isnan().all()
+        out[0, 2, 1] = clean[0, 2, 1]
+        assert t.equal(out, clean)
