@@ -302,7 +302,7 @@ __device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, co
 #pragma unroll
       for (int ks = 0; ks < DP / 32; ++ks) {
         const int e = 8 * (g4 + 4 * ks);
-        const V8 x = *reinterpret_cast<const V8*>(k + (e < a.head_dim ? e : 0));
+        const V8 x = e < a.head_dim ? *reinterpret_cast<const V8*>(k + e) : V8{};
 #pragma unroll
         for (int n = NS - 1; n >= 0; --n) s[t] = mfma16(x, q[ks][n], s[t]);
       }
@@ -355,7 +355,8 @@ __device__ __forceinline__ void store4(TO* p, f32x4 x, int left) {
 // T: cache type. NS: 16-bit terms of q and of the weights (1: q is of the cache's type; 2 / 3: q is float32, kept to 22 / 24
 // bits by terms of float16 / bfloat16, a weight too, float16's down to 2^-40 of the largest; with 1 term the weights are rounded
 // to the cache's type, half a step of it, as the output is). DP: head_dim rounded up to 64 / 128 / 256. FULL: it is DP itself;
-// else a piece behind head_dim is read at 0 instead (q is 0 there, and the output's dimensions behind it are not written).
+// else a piece behind head_dim is read at 0 instead (q and k are set to 0 there, and the output's dimensions behind it are not
+// written).
 // UNI: 16 consecutive keys from a multiple of 16 on lie in one page (page_size is a multiple of 16), so a page's address is a
 // scalar and a lane's place under it a constant 32-bit offset; else every lane looks up its own keys' pages.
 template <typename T, int NS, int DP, int RT, bool FULL, bool UNI>
@@ -439,6 +440,10 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 
   bool bad = false;
   for (; kt < k1; kt += 128) {
+    if constexpr (!FULL)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        if (8 * (g4 + 4 * ks) >= D) kr[0][ks] = kr[1][ks] = V8{};  // (as in q: an infinity there would make NaN)
     f32x4 s[RT][1][2];  // 32 keys x rows
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) s[rt][0][0] = s[rt][0][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -630,6 +635,10 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
     const bool drafted = kt + KT > L.ctx;
     const bool masked = drafted || present != (KT == 64 ? ~0ull : (1ull << KT) - 1);
     uint32_t bits[RT][KG];
+    if (D != DP)  // a piece behind head_dim: 0, as in q (an infinity there would make NaN)
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (8 * piece >= D) kr[i] = V8{};
     if (masked) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {

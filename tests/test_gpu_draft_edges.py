@@ -1,11 +1,11 @@
 """The drafted-token operators (fun_asr_gguf.ops) on the GPU where they can go wrong: many splits of narrow heads, infinities and
-NaN among committed keys, weights far below the largest, float32 queries of any size. Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
+NaN among keys, weights far below the largest, float32 queries of any size. Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
 import numpy as np
 import pytest
 import torch  # noqa: F401  (before any engine: the library then shares torch's HIP runtime)
 
 from draft_oracle import attention
-from test_gpu_draft_ops import check, close, kind, ops, paged, t, tolerance, trees, wide  # noqa: F401
+from test_gpu_draft_ops import U, check, close, kind, ops, paged, t, tolerance, trees, wide  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +113,36 @@ def test_attention_infinite_float32_queries(t, ops):
         assert out[0, 2, 1].isnan().all()
         out[0, 2, 1] = clean[0, 2, 1]
         assert t.equal(out, clean)
+
+
+@pytest.mark.parametrize("D,N,qn,cn", [
+    (96, 3, "f16", "f16"), (40, 40, "bf16", "bf16"), (80, 1, "bf16", "bf16"), (128, 4, "f16", "f16")])
+@pytest.mark.parametrize("whole", [False, True])
+def test_attention_infinite_keys(t, ops, D, N, qn, cn, whole):
+    """A score of -inf is a weight of 0, one of +inf a row of NaN, whatever lies beside the infinity in the products (`whole`:
+    queries of a few bits)."""
+    ctx = [70]
+    kc, vc, table = paged(t, ctx, N, 16, 2, D, cn, "hpd", 11)
+    g = t.Generator().manual_seed(2)
+    q = t.randint(1, 4, (1, N, 4, D), generator=g) * 0.5 if whole else t.randn(1, N, 4, D, generator=g).abs()
+    q[:, :, 1::2] *= -1  # one head of each pair meets +inf, the other -inf
+    q = q.to(kind(t, qn)).cuda()
+    lens = t.tensor(ctx, dtype=t.int32).cuda()
+    plain = lambda: attention(wide(q), np.where(np.isnan(wide(kc)), 0, wide(kc)), np.nan_to_num(wide(vc)),  # noqa: E731
+                              table.cpu().numpy(), ctx, [N], None, D ** -0.5)
+    _, mass, reach = plain()
+    tol = tolerance(0, mass, reach, qn, cn, D)
+    for p, d, what in ((10, 0, float("inf")), (10, D - 1, float("-inf")), (69, 1, float("inf")), (70, 5, float("-inf")),
+                       (64, 33, float("inf"))):
+        at = int(table[0, p // 16]), slice(None), p % 16
+        keep = kc[at].clone()
+        kc[at[0], :, at[2], d] = what
+        out = wide(ops.tree_attention(q, kc, vc, table, lens))
+        with np.errstate(invalid="ignore"):
+            want, _, _ = plain()
+        kc[at] = keep
+        none = np.isnan(want)
+        assert none.any() and not none.all()
+        assert (np.isnan(out) == none).all(), (p, d, what)
+        # (without the key the weights of the others grow, by no more than its share: the tolerance's mass does too)
+        assert (np.abs(out - want)[~none] <= (4 * tol + U[qn] * np.abs(want))[~none]).all(), (p, d, what)
