@@ -245,6 +245,23 @@ __device__ __forceinline__ void to_terms(const f32x4 (&s)[2], typename Vec8<T>::
   }
 }
 
+// With several terms of q an infinite key gives NaN where a lower term is 0, or of the other sign than the first: a score that
+// is NaN is made again, by f, from the first term alone, which tells infinity from NaN (and is all that counts beside infinity).
+// Rare, also where a key's place holds no key
+template <typename F>
+__device__ __forceinline__ void first_term_for_nan(f32x4 (&s)[2], F f) {
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) odd |= s[i >> 2][i & 3] != s[i >> 2][i & 3];
+  if (!__any(odd)) return;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const f32x4 x = f(t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[t][i] = s[t][i] == s[t][i] ? s[t][i] : x[i];
+  }
+}
+
 // eight elements at p + i. As a 32-bit offset in bytes under the pointer: where that is a scalar, the load adds them itself
 template <typename T>
 __device__ __forceinline__ typename Vec8<T>::type piece_at(const T* p, uint32_t i) {
@@ -288,7 +305,7 @@ __device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, co
   const float base = m == -INFINITY ? 0.f : base_of<T>(m, c);
   for (; kt < k1; kt += step) {
     if (kt + 32 <= L.ctx) continue;
-    f32x4 s[2];
+    const T* at[2];
     uint32_t present = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -297,16 +314,22 @@ __device__ __forceinline__ void add_nonfinite(const TreeP& P, const Where& w, co
       const int id = key < k1 ? table[pg] : -1;
       const bool ok = (uint32_t)id < (uint32_t)a.pages;
       present |= (uint32_t)(__ballot(ok) & 0xFFFF) << (16 * t);
-      const T* const k = ok ? kbase + id * a.k_page + (int64_t)((uint32_t)key - pg * a.page_size) * a.k_slot : kbase;
-      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      at[t] = ok ? kbase + id * a.k_page + (int64_t)((uint32_t)key - pg * a.page_size) * a.k_slot : kbase;
+    }
+    auto scores = [&](int t, int terms) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < DP / 32; ++ks) {
         const int e = 8 * (g4 + 4 * ks);
-        const V8 x = e < a.head_dim ? *reinterpret_cast<const V8*>(k + e) : V8{};
+        const V8 x = e < a.head_dim ? *reinterpret_cast<const V8*>(at[t] + e) : V8{};
 #pragma unroll
-        for (int n = NS - 1; n >= 0; --n) s[t] = mfma16(x, q[ks][n], s[t]);
+        for (int n = NS - 1; n >= 0; --n)
+          if (n < terms) s = mfma16(x, q[ks][n], s);
       }
-    }
+      return s;
+    };
+    f32x4 s[2] = {scores(0, NS), scores(1, NS)};
+    if constexpr (NS > 1) first_term_for_nan(s, [&](int t) { return scores(t, 1); });
     apply_mask(seen_bits(P, w.b, L.ctx, kt, present, node, g4), s);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -455,6 +478,15 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) s[rt][0][t] = mfma16(kr[t][ks], q[rt][ks][n], s[rt][0][t]);
+    if constexpr (NS > 1)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        first_term_for_nan(s[rt][0], [&](int t) {
+          f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) x = mfma16(kr[t][ks], q[rt][ks][0], x);
+          return x;
+        });
     const bool drafted = kt + 32 > L.ctx;  // the tile reaches the drafted keys or the end
     if (drafted || present != 0xFFFFFFFFu) {
 #pragma unroll
@@ -684,6 +716,19 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
         }
     }
     __builtin_amdgcn_s_setprio(0);
+    if constexpr (NS > 1)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+          first_term_for_nan(s[rt][g], [&](int t) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            const int key = 32 * g + 16 * t + r16;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+              x = mfma16(*reinterpret_cast<const V8*>(lk + key * DP + 8 * ((g4 + 4 * ks) ^ (key & (PIECES - 1)))), q[rt][ks][0], x);
+            return x;
+          });
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (masked)

@@ -116,11 +116,12 @@ def test_attention_infinite_float32_queries(t, ops):
 
 
 @pytest.mark.parametrize("D,N,qn,cn", [
-    (96, 3, "f16", "f16"), (40, 40, "bf16", "bf16"), (80, 1, "bf16", "bf16"), (128, 4, "f16", "f16")])
+    (96, 3, "f16", "f16"), (40, 40, "bf16", "bf16"), (80, 1, "bf16", "bf16"), (128, 4, "f16", "f16"),
+    (128, 3, "f32", "f16"), (128, 3, "f32", "bf16"), (64, 40, "f32", "f16"), (96, 2, "f32", "f16"), (256, 5, "f32", "bf16")])
 @pytest.mark.parametrize("whole", [False, True])
 def test_attention_infinite_keys(t, ops, D, N, qn, cn, whole):
-    """A score of -inf is a weight of 0, one of +inf a row of NaN, whatever lies beside the infinity in the products (`whole`:
-    queries of a few bits)."""
+    """A score of -inf is a weight of 0, one of +inf a row of NaN, whatever lies beside the infinity in the products: the places
+    behind a narrow head, or a float32 query's lower terms (`whole`: they are 0)."""
     ctx = [70]
     kc, vc, table = paged(t, ctx, N, 16, 2, D, cn, "hpd", 11)
     g = t.Generator().manual_seed(2)
@@ -146,3 +147,39 @@ def test_attention_infinite_keys(t, ops, D, N, qn, cn, whole):
         assert (np.isnan(out) == none).all(), (p, d, what)
         # (without the key the weights of the others grow, by no more than its share: the tolerance's mass does too)
         assert (np.abs(out - want)[~none] <= (4 * tol + U[qn] * np.abs(want))[~none]).all(), (p, d, what)
+
+
+@pytest.mark.parametrize("cn", ["f16", "bf16"])
+@pytest.mark.parametrize("D,N", [(128, 9), (96, 40)])
+@pytest.mark.parametrize("what", [float("inf"), float("-inf"), float("nan")])
+def test_attention_nonfinite_drafts_of_float32_queries(t, ops, cn, D, N, what):
+    """A drafted token's infinity reaches the tokens below it alone, in its value as in its key; another draft's key, infinite
+    too, is left out where its score is -inf."""
+    ctx = [45]
+    kc, vc, table = paged(t, ctx, N, 16, 2, D, cn, "hpd", 8)
+    q = t.randn(1, N, 4, D, generator=t.Generator().manual_seed(5)).cuda()
+    q[..., 3] = q[..., 3].abs() + 0.1
+    mask = trees(t, 1, N, 9)
+    mask[0, 8, 4] = True
+    seers = mask[0, :, 4]
+    lens = t.tensor(ctx, dtype=t.int32).cuda()
+    run = lambda: ops.tree_attention(q, kc, vc, table, lens, mask=mask.cuda())  # noqa: E731
+    check(t, ops, q, kc, vc, table, ctx, mask, names=("f32", cn))
+    gone = [int(table[0, 50 // 16]), slice(None), 50 % 16]  # draft 5: a score of -inf for every row
+    kc[(*gone, 3)] = float("-inf")
+    clean = run()
+    without = mask.clone()
+    without[0, :, 5] = False
+    assert t.equal(clean, ops.tree_attention(q, kc, vc, table, lens, mask=without.cuda()))  # (a weight of 0 either way)
+    at = int(table[0, 49 // 16]), slice(None), 49 % 16
+    for c, d in ((vc, 3), (vc, 77), (kc, 5)):
+        keep = c[at].clone()
+        c[(*at, d)] = what
+        out = run()
+        c[at] = keep
+        assert t.equal(out[0, ~seers], clean[0, ~seers])
+        if c is vc:
+            hit = out[0, seers][..., d]
+            assert hit.isnan().all() if what != what else (hit == what).all()
+            rest = [x for x in range(D) if x != d]
+            assert t.equal(out[0, seers][..., rest], clean[0, seers][..., rest])
