@@ -28,6 +28,7 @@
 #include "draft_ops.h"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace fa {
@@ -880,13 +881,18 @@ static TreePlan tree_plan(const fa_tree_attention_args* ap) {
   return t;
 }
 
-// a kernel's LDS beyond 64 KB has to be asked for, once
+// a kernel's LDS beyond 64 KB has to be asked for, once on every device; what fails is asked for again by the next call
 template <auto KERNEL, size_t LDS>
 static void tree_launch(const TreeP& P, hipStream_t s) {
   if constexpr (LDS > 65536) {
-    static const hipError_t once =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
-    FA_HIP(once);
+    static std::atomic<uint64_t> asked{0};  // a bit a device
+    int dev = 0;
+    FA_HIP(hipGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(asked.load(std::memory_order_relaxed) & bit)) {
+      FA_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS));
+      asked.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   launch(KERNEL, dim3((uint32_t)((P.n_groups + 7) / 8 * 8) * P.q_tiles), dim3(256), LDS, s, P);
 }

@@ -166,3 +166,46 @@ def test_tensors_that_require_a_gradient_are_refused():
     q = torch.zeros(2, 3, 32, requires_grad=True)
     with pytest.raises(ValueError, match="gradient"):
         ops.qk_norm_rope(q, q.detach(), None, None, None)
+
+
+def test_lds_is_asked_for_on_every_device(tmp_path):
+    """A kernel with more than 64 KB of LDS asks for it once on each device it runs on, and again where that failed. Four HIP
+    calls are replaced: the machine has the devices that the test says."""
+    import shutil
+    import subprocess
+    import sys
+    if not shutil.which("gcc"):
+        pytest.skip("no C compiler")
+    (tmp_path / "hip.c").write_text("""
+        static int device, fail, asked[8], launched;
+        void shim_set(int d, int f) { device = d; fail = f; }
+        int shim_asked(int d) { return asked[d]; }
+        int shim_launched(void) { return launched; }
+        int hipGetDevice(int* d) { *d = device; return 0; }
+        int hipDeviceGetAttribute(int* v) { *v = 256; return 0; }
+        int hipFuncSetAttribute() { if (fail) return 1; ++asked[device]; return 0; }
+        int hipLaunchKernel() { ++launched; return 0; }
+    """)
+    shim = str(tmp_path / "hip.so")
+    subprocess.run(["gcc", "-w", "-shared", "-fPIC", str(tmp_path / "hip.c"), "-o", shim], check=True)
+    here = os.path.dirname(os.path.abspath(__file__))
+    prog = f"""
+import ctypes, sys
+sys.path[:0] = [{here!r}, {os.path.join(os.path.dirname(here), "fun-asr-gguf_amd")!r}]
+from fun_asr_gguf import _native
+from test_draft_ops import tree
+lib, shim = _native.load(), ctypes.CDLL({shim!r})
+call = lambda: lib.fa_tree_attention(ctypes.byref(tree(head_dim=256, q_head=256, out_head=256, k_slot=256, v_slot=256)), None)
+for device in (0, 1):
+    shim.shim_set(device, 0)
+    assert call() == 0 and call() == 0, lib.fa_last_error()
+    assert shim.shim_asked(device) == 1, device
+shim.shim_set(2, 1)
+assert call() != 0 and shim.shim_launched() == 4
+shim.shim_set(2, 0)
+assert call() == 0 and shim.shim_asked(2) == 1 and shim.shim_launched() == 5
+print("fine")
+"""
+    env = dict(os.environ, LD_PRELOAD=":".join(x for x in (shim, os.environ.get("LD_PRELOAD")) if x))
+    r = subprocess.run([sys.executable, "-c", prog], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
