@@ -39,6 +39,7 @@ const at::Tensor* tensor(PyObject* o, const char* name) {
   NEED(THPVariable_Check(o), c10::str(name, " must be a tensor"));
   const at::Tensor& t = THPVariable_Unpack(o);
   NEED(!t.requires_grad() || !c10::GradMode::is_enabled(), c10::str(name, " requires a gradient: call under torch.no_grad()"));
+  NEED(!t._fw_grad(0).defined(), c10::str(name, " has a tangent: there is no forward-mode gradient"));
   NEED(!t.is_neg(), c10::str(name, " is a negated view"));
   return &t;
 }

@@ -209,3 +209,13 @@ print("fine")
     env = dict(os.environ, LD_PRELOAD=":".join(x for x in (shim, os.environ.get("LD_PRELOAD")) if x))
     r = subprocess.run([sys.executable, "-c", prog], capture_output=True, text=True, timeout=300, env=env)
     assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
+def test_tensors_with_a_tangent_are_refused():
+    import torch.autograd.forward_ad as fw
+    x, u = torch.zeros(2, 8), torch.zeros(2)
+    with fw.dual_level(), pytest.raises(ValueError, match="tangent"):
+        ops.sample_tokens(fw.make_dual(x, torch.ones(2, 8)), u)
+    q = torch.zeros(2, 3, 32)
+    with fw.dual_level(), pytest.raises(ValueError, match="tangent"):
+        ops.qk_norm_rope(fw.make_dual(q, q), q, None, None, None)
