@@ -39,7 +39,8 @@ const at::Tensor* tensor(PyObject* o, const char* name) {
   NEED(THPVariable_Check(o), c10::str(name, " must be a tensor"));
   const at::Tensor& t = THPVariable_Unpack(o);
   NEED(!t.requires_grad() || !c10::GradMode::is_enabled(), c10::str(name, " requires a gradient: call under torch.no_grad()"));
-  NEED(!t._fw_grad(0).defined(), c10::str(name, " has a tangent: there is no forward-mode gradient"));
+  NEED(!t.unsafeGetTensorImpl()->autograd_meta() || !t._fw_grad(0).defined(),
+       c10::str(name, " has a tangent: there is no forward-mode gradient"));
   NEED(!t.is_neg(), c10::str(name, " is a negated view"));
   return &t;
 }
@@ -51,6 +52,14 @@ const at::Tensor& gpu(PyObject* o, const char* name) {
 // a tensor that is written: no two elements in one place
 void written(const at::Tensor& t, const char* name) {
   NEED(at::has_internal_overlap(t) != at::MemOverlap::Yes, c10::str(name, " has elements that share memory"));
+}
+// a caller's tensor after the call: autograd notices that one it has saved is another now (an inference tensor has no version, nor
+// is it saved)
+void changed(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void changed(PyObject* o) {
+  if (o != Py_None) changed(THPVariable_Unpack(o));
 }
 int type_of(const at::Tensor& t, const char* name) {
   switch (t.scalar_type()) {
@@ -177,6 +186,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
   a.k_out_head = ok.stride(1);
   OnDevice dev(k.device());
   check(norm_rope_fn(&a, dev.stream), "fa_qk_norm_rope");
+  changed(v[9]);
+  changed(v[10]);
   PyObject* r = PyTuple_New(2);
   if (!r) return nullptr;
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(oq));
@@ -237,7 +248,10 @@ PyObject* kv_append(PyObject*, PyObject* const* p, Py_ssize_t n) {
   a.slots_64 = slots.scalar_type() == at::kLong;
   OnDevice dev(d);
   check(append_fn(&a, dev.stream), "fa_kv_append");
+  changed(kc);
+  changed(vc);
   if (!q) Py_RETURN_NONE;
+  changed(p[13]);
   return THPVariable_Wrap(oq);
   END_HANDLE_TH_ERRORS
 }
@@ -323,6 +337,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* p, Py_ssize_t n) {
   OnDevice dev(d);
   const at::Tensor ws = workspace(a, attention_ws_fn, "fa_tree_attention", d);
   check(attention_fn(&a, dev.stream), "fa_tree_attention");
+  changed(p[9]);
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
@@ -381,6 +396,8 @@ PyObject* sample_tokens(PyObject*, PyObject* const* p, Py_ssize_t n) {
   OnDevice dev(d);
   const at::Tensor ws = workspace(a, sample_ws_fn, "fa_sample_tokens", d);
   check(sample_fn(&a, dev.stream), "fa_sample_tokens");
+  changed(p[6]);
+  changed(p[7]);
   PyObject* r = PyTuple_New(2);
   if (!r) return nullptr;
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));

@@ -183,3 +183,28 @@ def test_attention_nonfinite_drafts_of_float32_queries(t, ops, cn, D, N, what):
             assert hit.isnan().all() if what != what else (hit == what).all()
             rest = [x for x in range(D) if x != d]
             assert t.equal(out[0, seers][..., rest], clean[0, seers][..., rest])
+
+
+def test_what_autograd_sees(t, ops):
+    """Every tensor that a call writes has a new version, so a graph that saved it notices; what it reads keeps its own."""
+    x = t.randn(1, 2, 4, 32, device="cuda", dtype=t.float16)
+    c, n = t.zeros(1, 2, 8, 32, device="cuda", dtype=t.float16), t.zeros(1, device="cuda", dtype=t.int32)
+    kc, vc, q, k = c.clone(), c.clone(), t.randn(4, 2, 32, device="cuda"), t.randn(4, 2, 32, device="cuda")
+    oq, ok, oa = t.empty_like(q), t.empty_like(k), t.empty_like(x)
+    tok, prob = t.zeros(2, device="cuda", dtype=t.int32), t.zeros(2, device="cuda")
+    logits, u = t.randn(2, 50, device="cuda"), t.rand(2, device="cuda")
+    written, read = [kc, vc, oq, ok, oa, tok, prob], [q, k, x, n, logits, u]
+    was = [a._version for a in written], [a._version for a in read]
+    ops.qk_norm_rope(q, k, None, None, None, out_q=oq, out_k=ok)
+    ops.kv_append(k, k, kc, vc, t.arange(4, device="cuda"))
+    ops.tree_attention(x, kc, vc, n.view(1, 1), n, out=oa)
+    ops.sample_tokens(logits, u, out=tok, out_prob=prob)
+    assert all(a._version > b for a, b in zip(written, was[0])) and [a._version for a in read] == was[1]
+    y = t.ones_like(kc, requires_grad=True)
+    z = (y * kc).sum()
+    ops.kv_append(k, k, kc, vc, t.arange(4, device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        z.backward()
+    with t.inference_mode():
+        i = t.zeros(1, 2, 8, 32, device="cuda", dtype=t.float16)
+        ops.kv_append(k, k, i, i.clone(), t.arange(4, device="cuda"))
