@@ -210,6 +210,8 @@ PyObject* kv_append(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const at::Tensor &k = gpu(p[0], "k"), &v = gpu(p[1], "v"), &kc = gpu(p[2], "k_cache"), &vc = gpu(p[3], "v_cache"),
                    &slots = gpu(p[4], "slots");
   const at::Tensor *cos = tensor(p[5], "cos"), *sin = tensor(p[6], "sin"), *pos = tensor(p[7], "positions"), *q = tensor(p[9], "q");
+  NEED(q || p[10] == Py_None, "q_weight without q");
+  NEED(q || p[13] == Py_None, "out_q without q");
   const at::Device d = k.device();
   fa_head_rows_args a{};
   head_args(a, k, q, cos, sin, pos, tensor(p[10], "q_weight"), tensor(p[8], "k_weight"), number(p[11], "eps"), truth(p[12]));

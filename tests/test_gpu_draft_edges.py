@@ -208,3 +208,13 @@ def test_what_autograd_sees(t, ops):
     with t.inference_mode():
         i = t.zeros(1, 2, 8, 32, device="cuda", dtype=t.float16)
         ops.kv_append(k, k, i, i.clone(), t.arange(4, device="cuda"))
+
+
+# ----------------------------------------------------------------------------------------------------------- arguments
+def test_arguments_that_would_be_ignored_are_refused(t, ops):
+    k = t.randn(4, 2, 32, device="cuda")
+    c, s, w = t.zeros(1, 2, 8, 32, device="cuda", dtype=t.float16), t.arange(4, device="cuda"), t.ones(32, device="cuda")
+    with pytest.raises(ValueError, match="out_q"):
+        ops.kv_append(k, k, c, c.clone(), s, out_q=t.empty_like(k))
+    with pytest.raises(ValueError, match="q_weight"):
+        ops.kv_append(k, k, c, c.clone(), s, q_weight=w)
