@@ -84,7 +84,11 @@ double number(PyObject* o, const char* name) {
   }
   return x;
 }
-int truth(PyObject* o) { return PyObject_IsTrue(o) > 0; }
+int truth(PyObject* o) {
+  const int x = PyObject_IsTrue(o);
+  if (x < 0) throw python_error();  // the object's own error (a tensor of several elements)
+  return x;
+}
 at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Device& d) {
   return at::Tensor(at::detail::empty_cuda(size, at::TensorOptions().dtype(type).device(d)));
 }

@@ -218,3 +218,12 @@ def test_arguments_that_would_be_ignored_are_refused(t, ops):
         ops.kv_append(k, k, c, c.clone(), s, out_q=t.empty_like(k))
     with pytest.raises(ValueError, match="q_weight"):
         ops.kv_append(k, k, c, c.clone(), s, q_weight=w)
+
+
+def test_an_interleaved_that_is_neither_true_nor_false_raises_its_own_error(t, ops):
+    k = t.randn(4, 2, 32, device="cuda")
+    with pytest.raises(RuntimeError, match="Boolean value"):
+        ops.qk_norm_rope(k, k, None, None, None, interleaved=t.zeros(2))
+    with pytest.raises(ZeroDivisionError):
+        ops.qk_norm_rope(k, k, None, None, None, interleaved=type("X", (), {"__bool__": lambda self: 1 // 0})())
+    assert all(t.equal(x, k) for x in ops.qk_norm_rope(k, k, None, None, None, interleaved=1))
