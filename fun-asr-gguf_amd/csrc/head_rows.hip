@@ -13,6 +13,8 @@
 #include "api.h"
 #include "draft_ops.h"
 
+#include <algorithm>
+
 namespace fa {
 
 struct HeadRowsP {
@@ -151,7 +153,7 @@ void head_rows(const fa_head_rows_args* ap, bool cache, hipStream_t s) {
     a.rot_dim = 0;
   }
   FA_REQUIRE(a.eps >= 0.f, "head rows: eps");
-  P.n_slots = a.heads + a.kv_heads * (cache ? 2 : 1);
+  const int64_t n_slots = a.heads + (int64_t)a.kv_heads * (cache ? 2 : 1);
   const bool some = a.tokens > 0;
   if (cache) {
     FA_REQUIRE(a.cache_type == FA_F16 || a.cache_type == FA_BF16, "kv_append: the cache is float16 or bfloat16");
@@ -174,8 +176,9 @@ void head_rows(const fa_head_rows_args* ap, bool cache, hipStream_t s) {
              "head rows: q in place with other strides");
   FA_REQUIRE(cache || a.k != a.k_out || !a.k || (a.k_token == a.k_out_token && a.k_head == a.k_out_head),
              "head rows: k in place with other strides");
-  FA_REQUIRE((int64_t)a.tokens * P.n_slots < (1ll << 31), "head rows: more than 2^31 rows");
-  if (!some || P.n_slots == 0) return;
+  FA_REQUIRE(std::max(a.tokens, 1) * n_slots < (1ll << 31), "head rows: more than 2^31 rows");  // (both below 2^33: no overflow)
+  P.n_slots = (int)n_slots;
+  if (!some || n_slots == 0) return;
   P.lpr = (uint32_t)a.head_dim / 16;
   P.lpr_div = FastDiv::of(P.lpr);
   P.wave_rows = 64 / P.lpr;

@@ -219,3 +219,10 @@ def test_tensors_with_a_tangent_are_refused():
     q = torch.zeros(2, 3, 32)
     with fw.dual_level(), pytest.raises(ValueError, match="tangent"):
         ops.qk_norm_rope(fw.make_dual(q, q), q, None, None, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(2 ** 31 - 1, 8), (8, 2 ** 31 - 1), (2 ** 30, 2 ** 30), (2 ** 31 - 1, 2 ** 31 - 1)])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_head_counts_whose_sum_passes_32_bits_are_refused(heads, kv_heads, tokens):
+    for call in ("fa_qk_norm_rope", "fa_kv_append"):
+        refused(call, head(heads=heads, kv_heads=kv_heads, tokens=tokens), "2^31")
