@@ -74,7 +74,7 @@ def tree_mask(parents):
     n = p.shape[-1]
     if not (bool((p < torch.arange(n)).all()) and bool((p >= -1).all())):
         raise ValueError("a node's parent must be an earlier node or -1")
-    flat = p.reshape(-1, n).long()
+    flat = p.reshape(p.shape[:-1].numel(), n).long()
     m = torch.zeros(flat.shape[0], n, n, dtype=torch.bool)
     for j in range(n):
         has = flat[:, j] >= 0

@@ -226,3 +226,11 @@ def test_tensors_with_a_tangent_are_refused():
 def test_head_counts_whose_sum_passes_32_bits_are_refused(heads, kv_heads, tokens):
     for call in ("fa_qk_norm_rope", "fa_kv_append"):
         refused(call, head(heads=heads, kv_heads=kv_heads, tokens=tokens), "2^31")
+
+
+def test_tree_mask_of_no_nodes_and_of_more_dimensions():
+    assert ops.tree_mask(torch.zeros(3, 0, dtype=torch.int32)).shape == (3, 0, 0)
+    assert ops.tree_mask([]).shape == (0, 0)
+    assert ops.tree_mask(torch.zeros(0, 4, dtype=torch.int64)).shape == (0, 4, 4)
+    p = torch.tensor([[[-1, 0, 1], [-1, -1, 0]]])
+    assert torch.equal(ops.tree_mask(p)[0, 1], ops.tree_mask([-1, -1, 0]))
