@@ -234,3 +234,27 @@ def test_tree_mask_of_no_nodes_and_of_more_dimensions():
     assert ops.tree_mask(torch.zeros(0, 4, dtype=torch.int64)).shape == (0, 4, 4)
     p = torch.tensor([[[-1, 0, 1], [-1, -1, 0]]])
     assert torch.equal(ops.tree_mask(p)[0, 1], ops.tree_mask([-1, -1, 0]))
+
+
+def test_the_engine_builds_without_torch(tmp_path):
+    """The binding of the operators is the one part that needs torch: without it the rest is built, and the engine's package
+    imports; the operators' module says what it misses."""
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    prog = f"""
+import sys
+sys.path[:0] = [{root!r}]
+sys.modules["torch"] = None  # (import torch raises ImportError)
+import __graft_entry__ as g
+assert g.build_ops() is None
+g.build_native = g.build_llama_compat = g._build_oracle_c = lambda: None
+g.build()
+import fun_asr_gguf
+try:
+    import fun_asr_gguf.ops
+except ImportError as e:
+    print("no operators:", e)
+"""
+    r = subprocess.run([sys.executable, "-c", prog], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "no operators" in r.stdout and "torch" in r.stderr, r.stdout + r.stderr
