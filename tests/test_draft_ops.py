@@ -258,3 +258,12 @@ except ImportError as e:
 """
     r = subprocess.run([sys.executable, "-c", prog], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "no operators" in r.stdout and "torch" in r.stderr, r.stdout + r.stderr
+
+
+def test_vocabularies_end_at_2_22():
+    """k_finish has a thread for every chunk up to there."""
+    lib, n = _native.load(), ctypes.c_int64()
+    refused("fa_sample_tokens", rows(vocab=2 ** 22 + 1, row_stride=2 ** 22 + 1), "2^22")
+    refused("fa_sample_tokens_workspace", rows(vocab=2 ** 22 + 1, row_stride=2 ** 22 + 1), "2^22", ctypes.byref(n))
+    assert lib.fa_sample_tokens_workspace(ctypes.byref(rows(vocab=2 ** 22, row_stride=2 ** 22)), ctypes.byref(n)) == 0
+    assert n.value > 2 * 1024 * 4

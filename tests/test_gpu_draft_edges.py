@@ -1,11 +1,12 @@
 """The drafted-token operators (fun_asr_gguf.ops) on the GPU where they can go wrong: many splits of narrow heads, infinities and
-NaN among keys, weights far below the largest, float32 queries of any size. Plain 64-bit forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
+NaN among keys, weights far below the largest, float32 queries of any size, large vocabularies, what autograd sees. Plain 64-bit
+forms: tests/draft_oracle.py; tolerances as in test_gpu_draft_ops.py unless a test says more."""
 import numpy as np
 import pytest
 import torch  # noqa: F401  (before any engine: the library then shares torch's HIP runtime)
 
 from draft_oracle import attention
-from test_gpu_draft_ops import U, check, close, kind, ops, paged, t, tolerance, trees, wide  # noqa: F401
+from test_gpu_draft_ops import U, check, close, kind, ops, paged, sampled, t, tolerance, trees, wide  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -227,3 +228,18 @@ def test_an_interleaved_that_is_neither_true_nor_false_raises_its_own_error(t, o
     with pytest.raises(ZeroDivisionError):
         ops.qk_norm_rope(k, k, None, None, None, interleaved=type("X", (), {"__bool__": lambda self: 1 // 0})())
     assert all(t.equal(x, k) for x in ops.qk_norm_rope(k, k, None, None, None, interleaved=1))
+
+
+# ------------------------------------------------------------------------------------------------------------ sampling
+@pytest.mark.parametrize("vocab", [151936, 200001, 262145, 2 ** 22])
+@pytest.mark.parametrize("kw", [dict(temperature=0.4, top_k=50), dict(top_k=5000, top_p=0.9), dict(top_p=0.95), dict(),
+                                dict(temperature=0.8, min_p=0.02), dict(temperature=0.0), dict(top_k=1000)])
+def test_sample_large_vocabularies(t, ops, vocab, kw):
+    """Up to the largest: more chunks than a wave has lanes, more maxima than k_finish holds in registers, a thread a chunk;
+    random numbers at both ends, rows at an odd stride."""
+    g = t.Generator(device="cuda").manual_seed(vocab)
+    u = t.tensor([0.37, 1 - 2.0 ** -24] if vocab == 2 ** 22 else [0.0, 0.37, 1 - 2.0 ** -24]).cuda()
+    big = t.randn(len(u), vocab + 5, device="cuda", generator=g) * 3
+    sampled(t, ops, big[:, 5:], u, **kw)
+    if vocab != 2 ** 22:
+        sampled(t, ops, big[1:2, :vocab].contiguous(), u[1:2], **kw)  # 16-byte aligned
