@@ -1764,7 +1764,8 @@ struct Engine {
     if (!small) prep_q8(latt, (int64_t)H * D, nullptr, lc.rms_eps, M, H * D, lxq2, lxd2, stream);
   }
 
-  // the drafts' forward, a draw at every row, the longest accepted path and its rows in the cache; returns the tokens gained
+  // the drafts' forward, a draw at every row, the accepted path (of children with the same token the first) and its rows in the
+  // cache; returns the tokens gained
   int verify(int seq, const int32_t* tokens, const int32_t* parents, int n, const fa_sampling* s, const float* u,
              int32_t* tokens_out, int32_t* path_out) {
     const int M = n + 1, E = lc.n_embd, V = lc.n_vocab;
@@ -1781,8 +1782,10 @@ struct Engine {
     a.token_out = vf_at<int>(0);  // over the rows' own tokens, which the embedding has read
     a.row_stride = V; a.rows = M; a.vocab = V; a.type = FA_F32;
     a.top_k = s ? s->top_k : 0; a.temperature = s ? s->temperature : 0.f; a.top_p = s ? s->top_p : 1.f;
+    // greedy: the generating step's own choice, from the LM head's maxima (a NaN logit ranks above every number there)
+    const bool greedy = !(a.temperature > 0.f) || a.top_k == 1;
     const fa_tree_attention_args t = vf_attention_args(M);
-    vf_reserve(std::max(tree_attention_bytes(&t), sample_tokens_bytes(&a)));
+    vf_reserve(std::max(tree_attention_bytes(&t), greedy ? 0 : sample_tokens_bytes(&a)));
     a.workspace = vf_ws; a.workspace_bytes = vf_ws_cap;
 
     std::vector<char> meta(VF_BYTES, 0);
@@ -1816,7 +1819,13 @@ struct Engine {
       throw;
     }
     vf_rows = 0;
-    sample_tokens(&a, stream);
+    if (greedy) {
+      set_sampling(nullptr);
+      sample_tokens(vf_logits, V, V, vf_pval, vf_pidx, n_part_cur, chunk_cur, M, d_samp, vf_at<int>(VF_SLOT), vf_at<int>(VF_POS),
+                    nullptr, a.token_out, nullptr, 0, nullptr, stream);
+    } else {
+      sample_tokens(&a, stream);
+    }
     std::vector<int> drawn(M);
     FA_HIP(hipMemcpyAsync(drawn.data(), vf_at<int>(0), (size_t)M * 4, hipMemcpyDeviceToHost, stream));
     FA_HIP(hipStreamSynchronize(stream));

@@ -204,12 +204,13 @@ int fa_llm_generate_end(fa_engine* e, int32_t* tokens_out);
 /* One decode step of sequence `seq` that also verifies n drafted tokens (0 .. 63), a tree whose root is the token that a
  * generate step would feed next: parents[i] is the index of draft i's parent, below i, or -1 for that token (NULL: a
  * chain). One forward over the n + 1 rows (fa_kv_append and fa_tree_attention on the engine's cache) gives every row its
- * next-token logits, and fa_sample_tokens draws from each with `s` (its seed is not used; NULL or temperature <= 0: the
- * largest logit) and u[row] in [0, 1), u [n + 1], row 0 the root's. From the root on, while a child holds the token drawn at
- * its parent, it is accepted. tokens_out [n + 1] receives the *n_out tokens drawn along the accepted path (at least one;
- * the last is what the next step feeds), path_out [n] (nullable) the accepted drafts' indices (*n_out - 1 of them). The
- * cache keeps the accepted rows alone, so the sequence goes on as if these tokens had been generated one by one: to the
- * decoder's noise floor, not bit for bit (other f32 summation orders). */
+ * next-token logits. With s NULL, temperature <= 0 or top_k 1 each row's token is the one that a generate step takes (the
+ * largest logit; a NaN above every number); else fa_sample_tokens draws from each with `s` (its seed is not used; a NaN counts
+ * as -inf, and a row with nothing above -inf is an error) and u[row] in [0, 1), u [n + 1], row 0 the root's. From the root on,
+ * while a child (of several, the first) holds the token drawn at its parent, it is accepted. tokens_out [n + 1] receives the
+ * *n_out tokens drawn along the accepted path (at least one; the last is what the next step feeds), path_out [n] (nullable) the
+ * accepted drafts' indices (*n_out - 1 of them). The cache keeps the accepted rows alone, so the sequence goes on as if these
+ * tokens had been generated one by one: to the decoder's noise floor, not bit for bit (other f32 summation orders). */
 int fa_llm_verify(fa_engine* e, int32_t seq, const int32_t* tokens, const int32_t* parents, int32_t n, const fa_sampling* s,
                   const float* u, int32_t* tokens_out, int32_t* path_out, int32_t* n_out);
 /* Logits [n_vocab] of sequence `seq` from the most recent forward (fa_llm_prefill, or the last step of

@@ -185,3 +185,35 @@ def test_entry_refuses_without_an_engine():
     lib, n = _native.load(), ctypes.c_int32(-7)
     assert lib.fa_llm_verify(None, 0, None, None, 0, None, None, None, None, ctypes.byref(n)) == -1
     assert n.value == -7 and b"fa_llm_verify" in lib.fa_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("samp", [dict(temperature=0.0), dict(temperature=0.7, top_k=1)])
+def test_greedy_is_that_of_the_generating_step_whatever_the_logits(samp):
+    """A NaN logit ranks above every number in both, the lower id first; of logits that are all -inf or NaN one is taken."""
+    from fun_asr_gguf import _native
+    e = _native.Engine(synth.ENC_TINY, dict(synth.LLM_TINY, n_ctx=64, max_seqs=1), max_batch=1, max_samples=16000)
+    try:
+        e.synthetic_weights(0)
+        V, E = 4096, synth.LLM_TINY["n_embd"]
+        clean = e.get_tensor_q8_0("token_embd.weight", V * E)
+        embd = e.embd_rows(np.arange(9) * 31 + 5)
+        for bad in ([], [1234], [3000, 2999], range(V)):
+            w = clean.copy().reshape(V, E // 32, 34)
+            w[list(bad), 0, :2] = np.float16(np.nan).view(np.uint16).reshape(1).view(np.uint8)
+            e.set_tensor_q8_0("token_embd.weight", w.reshape(-1))
+            drafts = [7, 9, 11, 13, 15, 17, 19]
+            picked = []
+            for n in (None, 0, 1, 7):  # the generating step; one row, two, eight
+                e.llm_reset(0)
+                e.llm_prefill(0, embd)
+                e.llm_set_token(0, 77)
+                if n is None:
+                    picked.append(int(e.llm_generate([0], 1, **samp)[0, 0]))
+                else:
+                    picked.append(e.llm_verify(0, drafts[:n], [-1] * n, u=np.full(n + 1, 0.5), **samp)[0][0])
+            assert len(set(picked)) == 1, (list(bad)[:3], picked)
+            if len(bad):
+                assert picked[0] == min(bad)
+    finally:
+        e.close()
