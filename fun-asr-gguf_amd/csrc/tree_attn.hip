@@ -269,16 +269,16 @@ __device__ __forceinline__ typename Vec8<T>::type piece_at(const T* p, uint32_t 
   return *reinterpret_cast<const typename Vec8<T>::type*>(reinterpret_cast<const char*>(p) + i * 2u);
 }
 
-// sets the infinities and NaN among 8 values to 0; true if there were any
+// sets the infinities and NaN among 8 values to 0 where `own` is all ones (0: leaves them); true if it did
 template <typename T>
-__device__ __forceinline__ bool strip_nonfinite(typename Vec8<T>::type& v) {
+__device__ __forceinline__ bool strip_nonfinite(typename Vec8<T>::type& v, uint32_t own) {
   uint4 u = __builtin_bit_cast(uint4, v);
   constexpr uint32_t E = kExp<T>;
   uint32_t hit = 0;
   for (uint32_t* x : {&u.x, &u.y, &u.z, &u.w}) {
     const uint32_t lo = (*x & E) == E ? 0xFFFFu : 0u, hi = (*x >> 16 & E) == E ? 0xFFFF0000u : 0u;
-    hit |= lo | hi;
-    *x &= ~(lo | hi);
+    hit |= (lo | hi) & own;
+    *x &= ~((lo | hi) & own);
   }
   v = __builtin_bit_cast(typename Vec8<T>::type, u);
   return hit != 0;
@@ -493,10 +493,11 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const bool gone = !((present >> (16 * t + r16)) & 1);
+        const uint32_t own = kt + 16 * t + r16 >= L.ctx ? ~0u : 0u;  // a drafted key's (no branch: 60.5 -> 59.5 us, 32 sequences)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           if (gone) vr[t][ks] = V8{};  // whatever lies there must not meet a weight of 0
-          if (kt + 16 * t + r16 >= L.ctx) bad |= strip_nonfinite<T>(vr[t][ks]);
+          if (drafted) bad |= strip_nonfinite<T>(vr[t][ks], own);
         }
       }
 #pragma unroll
@@ -676,7 +677,7 @@ __global__ __launch_bounds__(256, DP == 256 || RT * NS > 2 || !UNI ? 1 : 2) void
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         if (!((present >> (i * KPS + row)) & 1)) vr[i] = V8{};
-        if (kt + i * KPS + row >= L.ctx) bad |= strip_nonfinite<T>(vr[i]);
+        if (drafted) bad |= strip_nonfinite<T>(vr[i], kt + i * KPS + row >= L.ctx ? ~0u : 0u);
       }
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
