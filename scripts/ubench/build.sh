@@ -2,7 +2,7 @@
 # Build the microbenchmarks against the engine's kernel objects (run from the repo root after build()).
 # VARIANT="-DNAME=value ..." builds decode_step_v / attn_stamps_v from llm.hip with those extra defines.
 set -e
-B=fun-asr-gguf_amd/build; U=scripts/ubench; F="-O3 -std=c++17 --offload-arch=gfx950 -Iinclude"
+B=fun-asr-gguf_amd/build; U=scripts/ubench; F="-O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude"
 hipcc $F -c $U/decode_step.hip -o /tmp/ds.o && hipcc --offload-arch=gfx950 /tmp/ds.o $B/llm.hip.o $B/synth.hip.o -o $U/decode_step
 hipcc $F $U/edge_chain.hip -o $U/edge_chain
 hipcc $F $U/kv_stream.hip -o $U/kv_stream

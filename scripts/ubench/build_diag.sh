@@ -4,7 +4,7 @@
 # attn_f32_bench_d{1..4} (FA_ATTN_DIAG: no K/V staging / no S MFMAs / no PV MFMAs / no softmax). They are
 # gpurun-ignored: drop them from .gpurunignore before a run that needs them.
 set -e
-B=fun-asr-gguf_amd/build; U=scripts/ubench; F="-O3 -std=c++17 --offload-arch=gfx950 -Iinclude"
+B=fun-asr-gguf_amd/build; U=scripts/ubench; F="-O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude"
 hipcc $F -c $U/gemm_f32_bench.hip -o /tmp/gf.o
 for v in 3 4; do
   hipcc $F -DB3B_VARIANT=$v -x hip -c fun-asr-gguf_amd/csrc/gemm_f32.hip -o /tmp/gemm_v$v.o

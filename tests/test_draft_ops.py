@@ -267,3 +267,21 @@ def test_vocabularies_end_at_2_22():
     refused("fa_sample_tokens_workspace", rows(vocab=2 ** 22 + 1, row_stride=2 ** 22 + 1), "2^22", ctypes.byref(n))
     assert lib.fa_sample_tokens_workspace(ctypes.byref(rows(vocab=2 ** 22, row_stride=2 ** 22)), ctypes.byref(n)) == 0
     assert n.value > 2 * 1024 * 4
+
+
+def test_every_script_builds_device_code_with_the_library_s_flags():
+    """A variant or a microbenchmark is compared with the library: no packed f32 instructions there either."""
+    import glob
+    import __graft_entry__ as g
+    flags = " ".join(g.HIP_FLAGS)
+    found = 0
+    for path in glob.glob(os.path.join(g.ROOT, "scripts", "**", "*.sh"), recursive=True):
+        text = open(path).read().replace("\\\n", " ")
+        for line in text.splitlines():
+            if "hipcc" not in line or line.lstrip().startswith("#"):
+                continue
+            for cmd in line.split("&&"):
+                if "hipcc" in cmd and ".hip" in cmd.replace(".hip.o", ""):  # (a link of objects compiles nothing)
+                    found += 1
+                    assert flags in cmd or ("$F" in cmd and flags in text[:text.index("hipcc")]), (path, cmd)
+    assert found > 10
