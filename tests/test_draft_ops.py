@@ -248,7 +248,7 @@ sys.path[:0] = [{root!r}]
 sys.modules["torch"] = None  # (import torch raises ImportError)
 import __graft_entry__ as g
 assert g.build_ops() is None
-g.build_native = g.build_llama_compat = g._build_oracle_c = lambda: None
+g.build_native = g.build_llama_compat = g._build_oracle_c = lambda **kw: None
 g.build()
 import fun_asr_gguf
 try:
@@ -285,3 +285,20 @@ def test_every_script_builds_device_code_with_the_library_s_flags():
                     found += 1
                     assert flags in cmd or ("$F" in cmd and flags in text[:text.index("hipcc")]), (path, cmd)
     assert found > 10
+
+
+def test_build_compiles_every_source_each_time(monkeypatch):
+    """build() is the check that the tree builds: nothing is skipped because an older result is there."""
+    import subprocess
+    import __graft_entry__ as g
+    if not os.path.exists(g.LIB):
+        pytest.skip("nothing built")
+    done = []
+
+    def run(cmd, **kw):
+        done.append(" ".join(map(str, cmd)))
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+    monkeypatch.setattr(g.subprocess, "run", run)
+    g.build()
+    for src in g.SOURCES + ["ops_torch.cpp", "llama_compat.cpp", "ggml_compat.c"]:
+        assert any(os.path.join(g.CSRC, src) + " " in c for c in done), src
