@@ -15,15 +15,18 @@
 //     wave-private LDS.
 //   k_many: the softmax's vector instructions weigh as much as the reading. The block's waves take 16 RT rows each and share
 //     every K and V tile through two LDS stages, so a tile is read once for 64 RT rows; one barrier a tile.
-// In LDS, row k's 16-byte piece j lies at j ^ (k mod pieces): an operand read's 16 rows, and a transposing read's 16 rows of
-// 32 bytes, then cover all banks evenly.
+// In LDS, row k's 16-byte piece j lies at j ^ (k mod pieces), which spreads rows over the banks, but not quite evenly: for heads
+// over 64, half a wave's transposing read holds keys 0-7 with pieces 2 m and 2 m + 1, and keys k and k ^ 1 meet on one pair of
+// banks; for heads up to 64 the operand read of K does so. Counted: 25 % of k_many's LDS cycles are conflicts, of k_few's 19 (32
+// sequences) and 24 % (one token a sequence).
 // Blocks of the same rows split the keys where the launch would not fill the card; k_tree_merge joins their partial results
 // (unnormalised output, base, sum).
 //
 // Measured: 48 sequences of up to 8191 keys, one token each, 32 / 8 heads of 128: 206 us, 5.0 TB/s of K and V; 32 of up to 2032
 // keys, 16 drafted tokens, 16 / 8 heads: 54 + 6 us (blocks of 1024 keys begin and end for a fifth of it); 4 of 32685 keys, 63
 // drafted tokens, 32 / 8 heads (k_many): 201 us, 670 TFLOP/s, the matrix units busy a third of the time, the waves waiting for
-// operands a third; 8 tokens on 212 keys: 10 us, the chain lengths, page, K, products, V, join.
+// operands a third (60 calls back to back: 207 at first, up to 268 in between, 211 at the end); 8 float32 tokens on 212 keys:
+// 10.4 us, the chain lengths, page, K, products, V, join.
 #include "api.h"
 #include "draft_ops.h"
 

@@ -11,6 +11,9 @@ gradient: a tensor that requires one is refused outside torch.no_grad(). Outputs
 A program that also creates an Engine imports torch (or this module) before the first one: torch brings a HIP runtime of its
 own, and the engine's library uses it where it is loaded already. The other way round the process holds two, and torch's
 finds no device.
+
+Tensors that a call writes (caches, out, out_q ...) get a new version, as by any in-place operation of torch. A tensor with a
+forward-mode tangent is refused.
 """
 import ctypes
 import importlib.machinery
@@ -62,7 +65,8 @@ def kv_append(k, v, k_cache, v_cache, slots, *, cos=None, sin=None, positions=No
     """k (normed and rotated as in qk_norm_rope) and v [tokens, kv_heads, head_dim] into the pages of a cache: k_cache /
     v_cache [pages, kv_heads, page_size, head_dim] of float16 or bfloat16 (any strides that keep rows 16-byte aligned), token
     t at slots[t] = page * page_size + offset. A token with a slot outside the cache (padding: -1) is not appended. The
-    slots of one call are distinct. q: its rows are normed and rotated in the same launch. -> q's rows (None without q)"""
+    slots of one call are distinct. q: its rows are normed and rotated in the same launch (q_weight and out_q belong to it).
+    -> q's rows (None without q)"""
     return (_module or _ops()).kv_append(k, v, k_cache, v_cache, slots, cos, sin, positions, k_weight, q, q_weight, eps, interleaved,
                                          out_q)
 
@@ -90,7 +94,8 @@ def tree_attention(q, k_cache, v_cache, block_table, context_lens, *, mask=None,
     block_table[b, p // page_size] (int32 [seqs, width]); it has context_lens[b] (int32) committed tokens and behind them
     draft_lens[b] (int32; None: nodes) drafted ones, already appended. Drafted token i sees all committed tokens and the
     drafted tokens j with mask[.., i, j] (bool [nodes, nodes] or [seqs, nodes, nodes], see tree_mask; None: j <= i, so one
-    node is an ordinary decoding step). A row that sees nothing is 0; rows behind draft_lens[b] are left as they were.
+    node is an ordinary decoding step). A row that sees nothing is 0; rows behind draft_lens[b] are left as they were. Weights
+    are rounded to the cache's type for the second product; float32 q keeps them, and q itself, to 22 (float16 cache) or 24 bits.
     max_context: the largest context length if the caller knows it (default: what the table holds); it shapes the launch,
     not the result's definition. scale: default head_dim ** -0.5. -> out, like q"""
     return (_module or _ops()).tree_attention(q, k_cache, v_cache, block_table, context_lens, mask, draft_lens, scale, max_context,

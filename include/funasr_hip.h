@@ -326,12 +326,19 @@ int fa_kv_append(const fa_head_rows_args* a, void* stream);
  * logical positions context_lens[b] + j. Key position p of sequence b lies in page block_table[b][p / page_size] at
  * offset p % page_size. Drafted token i sees every committed key and the drafted keys j with mask[b][i][j] != 0
  * (NULL: j <= i, so nodes = 1 is an ordinary decoding step and a chain is verified or prefilled causally):
- *   out[b][i] = softmax_j(scale * q[b][i] . k[j]) v[j], statistics in 32 bits; a row that sees no key is 0.
- * q / out [seqs, nodes, heads, head_dim], head h reads kv head h / (heads / kv_heads). q_type is cache_type, or FA_F32
- * (then q and the probabilities enter the products as sums of 16-bit terms, which keeps 32-bit accuracy). head_dim is a
- * multiple of 8, at most 256. Rows of out with i >= draft_lens[b] are left as they were. Lengths are cut to what the
- * block table holds; a page number outside [0, pages) makes its keys absent. max_context bounds context_lens for the
- * split of long sequences over the card (a longer one is still computed right, only slower). */
+ *   out[b][i] = softmax_j(scale * q[b][i] . k[j]) v[j]; a row that sees no key is 0.
+ * q / out [seqs, nodes, heads, head_dim], head h reads kv head h / (heads / kv_heads). head_dim is a multiple of 8, at most 256.
+ * q_type is cache_type, or FA_F32. Scores, maxima, sums and the output's sums are in 32 bits; the weights enter the second
+ * product rounded to the cache's type (2^-11 of a weight over FA_F16, 2^-8 over FA_BF16), as the output is at the end. With
+ * FA_F32, q and the weights enter the products as sums of 16-bit terms: a row of q, whatever its size, to 2^-22 of each element
+ * over FA_F16 (never finer than 2^-39 of the row's largest), 2^-24 over FA_BF16, the weights likewise. Over FA_F16 no weight is
+ * finer than 2^-40 of its row's largest, so that n keys far below it can shift the output by n 2^-40 of the largest value.
+ * Infinities and NaN: a key with a score of -inf has no weight (a row with no others is 0), a score of +inf or NaN makes its row
+ * NaN. A value's infinity or
+ * NaN reaches the rows that see its key, and no others (NaN for infinity where a committed key's weight is rounded to 0).
+ * Rows of out with i >= draft_lens[b] are left as they were. Lengths are cut to what the block table holds; a page number
+ * outside [0, pages) makes its keys absent. max_context bounds context_lens for the split of long sequences over the card (a
+ * longer one is still computed right, only slower). */
 typedef struct fa_tree_attention_args {
   const void* q;
   void* out;
