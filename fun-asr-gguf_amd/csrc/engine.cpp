@@ -1704,7 +1704,8 @@ struct Engine {
   // ---- verification of drafted tokens (fa_llm_verify)
   // byte offsets of vf_meta
   static constexpr int VF_POS = VF_MAX * 4, VF_SLOT = VF_MAX * 8, VF_U = VF_MAX * 12, VF_SEQ = VF_MAX * 16,
-                       VF_MASK = VF_MAX * 16 + 16, VF_BYTES = VF_MASK + VF_MAX * VF_MAX;
+                       VF_GREEDY = VF_MAX * 16 + 16,  // SampleParams of zeros: the largest logit
+                       VF_MASK = VF_GREEDY + (int)sizeof(SampleParams), VF_BYTES = VF_MASK + VF_MAX * VF_MAX;
   template <class T>
   T* vf_at(int byte) { return reinterpret_cast<T*>(reinterpret_cast<char*>(vf_meta) + byte); }
 
@@ -1820,9 +1821,8 @@ struct Engine {
     }
     vf_rows = 0;
     if (greedy) {
-      set_sampling(nullptr);
-      sample_tokens(vf_logits, V, V, vf_pval, vf_pidx, n_part_cur, chunk_cur, M, d_samp, vf_at<int>(VF_SLOT), vf_at<int>(VF_POS),
-                    nullptr, a.token_out, nullptr, 0, nullptr, stream);
+      sample_tokens(vf_logits, V, V, vf_pval, vf_pidx, n_part_cur, chunk_cur, M, vf_at<SampleParams>(VF_GREEDY), vf_at<int>(VF_SLOT),
+                    vf_at<int>(VF_POS), nullptr, a.token_out, nullptr, 0, nullptr, stream);
     } else {
       sample_tokens(&a, stream);
     }
